@@ -253,6 +253,80 @@ int moe_fp8_block_scale_route_static(const float* routing_logits, const uint16_t
                                      int32_t* topk_idx, float* topk_w, int32_t* expert_offsets,
                                      int32_t* perm_token, float* perm_weight, void* stream);
 
+/* ---- Operators around the shard: what a decoder layer does directly before the router and the experts and directly
+ * after them.  No counterparts in the reference.  All are asynchronous on `stream`, can be captured in a CUDA graph,
+ * keep nothing between calls, take device pointers and give the same bits for the same inputs.  Tensors carry a type
+ * code; a stride is the distance of two rows in elements, the elements of a row are adjacent, outputs are contiguous. */
+#define MOE_B200_F32 0
+#define MOE_B200_BF16 1
+#define MOE_B200_F16 2
+
+/* Norms before and after a block with the block's gate and the residual scale in one pass over the rows:
+ *   r1 = rsqrt(mean(y^2) + eps)    n = y * r1 * post_weight           (n = y without post_weight)
+ *   s  = residual_scale * x + gate * n                                (s = x without y)
+ *   r2 = rsqrt(mean(s^2) + eps)    h = s * r2 * pre_weight
+ *   x, y [T, H] (y may be NULL), H <= 16384; pre_weight [H]; post_weight [H] or NULL (needs y)
+ *   gate_kind 0: none, 1: [H] per channel, 2: [T] per token (gate_stride apart), 3: [T, H]; needs y
+ *   param_f32: bit 0 / 1 / 2 set: pre_weight / post_weight / gate are fp32, else they have x's type
+ *   stream_out [T, H] = s (only with y); rstd f32 [T, 2] = (r1 or 0, r2), which the backward takes
+ *   h_scale NULL: h [T, H] in x's type.  h_scale given: the shard's input, h e4m3 [T, H] and h_scale f32 [H / 128, T]
+ *   (max(|h|, 1e-10) / 448 per 128 columns, from the unrounded h); H a multiple of 128, rows 16-byte aligned.
+ * Everything in between is fp32; what is stored is rounded once, h comes from the unrounded s. */
+int moe_fp8_block_scale_block_norm(const void* x, int64_t x_stride, const void* y, int64_t y_stride, const void* gate,
+                                   int64_t gate_stride, int gate_kind, const void* pre_weight, const void* post_weight,
+                                   int T, int H, int dtype, int param_f32, float residual_scale, float eps,
+                                   void* stream_out, void* h, float* h_scale, float* rstd, void* stream);
+
+/* Its gradients.  grad_h [T, H] belongs to h (straight through the quantisation), grad_stream [T, H] or NULL to s.
+ * grad_x, grad_y (with y), grad_gate (the gate's shape, contiguous), grad_pre_weight, grad_post_weight have the types of
+ * what they belong to.  Sums over tokens are fp32 in a fixed order, in `workspace` (16-byte aligned).  T == 0 returns at
+ * once and writes nothing. */
+size_t moe_fp8_block_scale_block_norm_backward_workspace_bytes(int T, int H);
+int moe_fp8_block_scale_block_norm_backward(const void* x, int64_t x_stride, const void* y, int64_t y_stride,
+                                            const void* gate, int64_t gate_stride, int gate_kind,
+                                            const void* pre_weight, const void* post_weight, int T, int H, int dtype,
+                                            int param_f32, float residual_scale, const float* rstd, const void* grad_h,
+                                            int64_t grad_h_stride, const void* grad_stream, int64_t grad_stream_stride,
+                                            void* grad_x, void* grad_y, void* grad_gate, void* grad_pre_weight,
+                                            void* grad_post_weight, void* workspace, size_t workspace_bytes,
+                                            void* stream);
+
+/* Balance loss of a routing per sequence, with per-expert counts: p = s / sum(s) over a token's E experts with
+ * s = sigmoid(logits) or exp(logits); for a sequence with n counted tokens, c_i selections of expert i among them,
+ *   loss = alpha * E / (K n^2) * sum_i c_i sum_t p_ti          (0 for a sequence without a counted token)
+ *   logits [T, E], E <= 1024; topk_idx i32 [T, K] contiguous (an index outside [0, E) counts nowhere)
+ *   cu_seqlens i32 [S + 1]: sequence q has tokens cu_seqlens[q] .. cu_seqlens[q + 1] - 1 (ascending; tokens outside
+ *   every sequence are not read), or NULL with S == 1: one sequence of T tokens
+ *   token_mask u8 [T] or NULL: tokens with 0 are not read
+ *   loss f32 [S], counts i32 [S, E], tokens i32 [S] (counted tokens).
+ * Borders outside [0, T] are read as 0 or T; borders that descend give undefined results but no access out of range. */
+#define MOE_B200_SCORE_SIGMOID 0
+#define MOE_B200_SCORE_SOFTMAX 1
+size_t moe_fp8_block_scale_balance_loss_workspace_bytes(int T, int E);
+int moe_fp8_block_scale_balance_loss(const void* logits, int64_t logits_stride, int dtype, const int32_t* topk_idx, int T,
+                                     int E, int K, const int32_t* cu_seqlens, int S, const uint8_t* token_mask,
+                                     int scoring, float alpha, float* loss, int32_t* counts, int32_t* tokens,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its gradient for the logits, with the counts constant: grad_logits [T, E] in the logits' type, zero for tokens that
+ * are masked or in no sequence.  grad_loss f32 [S]; counts and tokens as the forward left them. */
+int moe_fp8_block_scale_balance_loss_backward(const float* grad_loss, const void* logits, int64_t logits_stride, int dtype,
+                                              const int32_t* counts, const int32_t* tokens, int T, int E, int K,
+                                              const int32_t* cu_seqlens, int S, const uint8_t* token_mask, int scoring,
+                                              float alpha, void* grad_logits, void* stream);
+
+/* Products of up to 256 (row, expert) pairs with 4-bit weights and group scales:
+ *   out[p, n] = sum_k x[p / pairs_per_row, k] * (q[e, n, k] - z[e, n, k / G]) * scale[e, n, k / G],   e = experts[p]
+ *   x [pairs / pairs_per_row, K], bf16 or fp16, rows 16-byte aligned; qweight u8 [E, N, K / 2]: two values a byte, the
+ *   even k in the low half, 16-byte aligned; scale [E, N, K / G] in x's type or fp32 (scale_f32); zero u8 [E, N, K / G]
+ *   with values 0..15, or NULL: 8; G 32, 64 or 128, K a multiple of G
+ *   experts i32 [pairs]: an expert outside [0, E) is not held here, its row of out is zero; NULL with E == 1 and
+ *   pairs_per_row == 1: one matrix for all rows
+ *   out [pairs, N] in x's type or fp32 (out_f32).  Sums are fp32; a weight's q - z is exact. */
+int moe_fp8_block_scale_matvec_w4(const void* x, int64_t x_stride, int dtype, const uint8_t* qweight, const void* scale,
+                                  int scale_f32, const uint8_t* zero, const int32_t* experts, int pairs,
+                                  int pairs_per_row, int E, int N, int K, int G, void* out, int out_f32, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -37,7 +37,16 @@ EXPORTS = [
     "moe_ep_plan",
     "moe_ep_row_pointers",
     "moe_ep_quantize_push",
+    "moe_fp8_block_scale_block_norm",
+    "moe_fp8_block_scale_block_norm_backward",
+    "moe_fp8_block_scale_block_norm_backward_workspace_bytes",
+    "moe_fp8_block_scale_balance_loss",
+    "moe_fp8_block_scale_balance_loss_backward",
+    "moe_fp8_block_scale_balance_loss_workspace_bytes",
+    "moe_fp8_block_scale_matvec_w4",
 ]
+F32, BF16, F16 = 0, 1, 2                       # type codes of the operators around the shard
+SCORE_SIGMOID, SCORE_SOFTMAX = 0, 1
 STATIC_MAX_TOKENS = 4096
 STAGES = ("route_permute", "gather", "gemm1", "swiglu_split", "gemm2", "combine")
 
@@ -116,6 +125,25 @@ def _load() -> ctypes.CDLL:
     lib.moe_fp8_block_scale_launch_count.argtypes = []
     lib.moe_fp8_block_scale_set_profiling.restype = i32
     lib.moe_fp8_block_scale_set_profiling.argtypes = [i32]
+    i64 = ctypes.c_int64
+    lib.moe_fp8_block_scale_block_norm.restype = i32
+    lib.moe_fp8_block_scale_block_norm.argtypes = \
+        [vp, i64, vp, i64, vp, i64, i32, vp, vp, i32, i32, i32, i32, f32, f32, vp, vp, vp, vp, vp]
+    lib.moe_fp8_block_scale_block_norm_backward_workspace_bytes.restype = sz
+    lib.moe_fp8_block_scale_block_norm_backward_workspace_bytes.argtypes = [i32, i32]
+    lib.moe_fp8_block_scale_block_norm_backward.restype = i32
+    lib.moe_fp8_block_scale_block_norm_backward.argtypes = \
+        [vp, i64, vp, i64, vp, i64, i32, vp, vp, i32, i32, i32, i32, f32, vp, vp, i64, vp, i64] + [vp] * 6 + [sz, vp]
+    lib.moe_fp8_block_scale_balance_loss_workspace_bytes.restype = sz
+    lib.moe_fp8_block_scale_balance_loss_workspace_bytes.argtypes = [i32, i32]
+    lib.moe_fp8_block_scale_balance_loss.restype = i32
+    lib.moe_fp8_block_scale_balance_loss.argtypes = \
+        [vp, i64, i32, vp, i32, i32, i32, vp, i32, vp, i32, f32, vp, vp, vp, vp, sz, vp]
+    lib.moe_fp8_block_scale_balance_loss_backward.restype = i32
+    lib.moe_fp8_block_scale_balance_loss_backward.argtypes = \
+        [vp, vp, i64, i32, vp, vp, i32, i32, i32, vp, i32, vp, i32, f32, vp, vp]
+    lib.moe_fp8_block_scale_matvec_w4.restype = i32
+    lib.moe_fp8_block_scale_matvec_w4.argtypes = [vp, i64, i32, vp, vp, i32, vp, vp] + [i32] * 6 + [vp, i32, vp]
     lib.moe_fp8_block_scale_stage_times.restype = i32
     lib.moe_fp8_block_scale_stage_times.argtypes = [ctypes.POINTER(f32), i32]
     return lib

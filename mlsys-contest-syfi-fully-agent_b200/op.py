@@ -240,6 +240,288 @@ def quantize_activations(hidden_bf16: torch.Tensor):
     return q, s
 
 
+# ---------------------------------------------------------------------------- operators around the shard
+#
+# What a decoder layer does directly before the router and the experts and directly after them.  Like ``run`` they work
+# on torch's current stream of the tensors' device and can be captured in a CUDA graph; they record nothing for
+# autograd: every gradient is a call of its own.  Scratch memory comes from torch's allocator for the call.
+
+_TYPE_CODE = {torch.float32: loader.F32, torch.bfloat16: loader.BF16, torch.float16: loader.F16}
+_SCORING = {"sigmoid": loader.SCORE_SIGMOID, "softmax": loader.SCORE_SOFTMAX}
+NORM_MAX_WIDTH, BALANCE_MAX_EXPERTS, MATVEC_MAX_PAIRS = 16384, 1024, 256
+_scratch_bytes: Dict[tuple, int] = {}          # library's workspace size per kind and sizes
+
+
+def _scratch(kind, fn, a: int, b: int, dev: torch.device) -> torch.Tensor:
+    need = _scratch_bytes.get((kind, a, b))
+    if need is None:
+        if len(_scratch_bytes) >= 4096:
+            _scratch_bytes.clear()
+        need = _scratch_bytes[kind, a, b] = int(fn(a, b))
+    return torch.empty(need, dtype=torch.uint8, device=dev)
+
+
+def _rows(name: str, t: torch.Tensor, T: int, H: int, dtype: torch.dtype, dev: torch.device):
+    """Checks an activation argument [T, H] whose rows may lie apart; returns (address, row stride)."""
+    _check(t.dtype == dtype and t.dim() == 2 and t.shape[0] == T and t.shape[1] == H and t.device == dev,
+           f"{name} must be {dtype} [{T}, {H}] on {dev}")
+    stride = t.stride()
+    _check(stride[1] == 1 or H <= 1, f"{name}: the elements of a row must be adjacent")
+    return t.data_ptr(), stride[0] if T > 1 else 0
+
+
+def _aligned(t: Optional[torch.Tensor]) -> bool:
+    """Rows (or the one row) of an argument can be read 16 bytes at a time."""
+    return t is None or (t.data_ptr() % 16 == 0 and
+                         (t.dim() == 1 or t.shape[0] <= 1 or t.stride(0) * t.element_size() % 16 == 0))
+
+
+def _on_gpu(t: torch.Tensor):
+    _check(t.is_cuda, "the tensors must be on a GPU: there is no CPU path")
+
+
+def _param(name: str, t: torch.Tensor, H: int, dtype: torch.dtype, dev: torch.device):
+    """Checks a parameter [H] in the activations' type or float32; returns (address, is float32)."""
+    _check((t.dtype == dtype or t.dtype == torch.float32) and t.dim() == 1 and t.shape[0] == H and
+           t.device == dev and (H <= 1 or t.stride(0) == 1), f"{name} must be a contiguous {dtype} or float32 [{H}] on {dev}")
+    return t.data_ptr(), t.dtype == torch.float32
+
+
+def _norm_inputs(x, pre_weight, y, post_weight, gate, residual_scale):
+    """Checks what both directions of the block norm take; returns the leading arguments of the C call."""
+    code = _TYPE_CODE.get(x.dtype)
+    _check(code is not None and x.dim() == 2, "x must be float32, bfloat16 or float16 [T, H]")
+    T, H = x.shape
+    _check(1 <= H <= NORM_MAX_WIDTH and T < 2 ** 31, f"x must have 1 to {NORM_MAX_WIDTH} columns")
+    dtype, dev = x.dtype, x.device
+    xp, xs = _rows("x", x, T, H, dtype, dev)
+    pre, f32 = _param("pre_weight", pre_weight, H, dtype, dev)
+    params = 1 if f32 else 0
+    yp = ys = post = gp = gs = kind = 0
+    if y is not None:
+        yp, ys = _rows("y", y, T, H, dtype, dev)
+        if post_weight is not None:
+            post, f32 = _param("post_weight", post_weight, H, dtype, dev)
+            params |= 2 if f32 else 0
+        if gate is not None:
+            if gate.dim() == 1:
+                gp, f32 = _param("gate", gate, H, dtype, dev)
+                kind = 1
+            else:
+                f32 = gate.dtype == torch.float32
+                per_token = gate.dim() == 2 and gate.shape[1] == 1
+                gp, gs = _rows("gate", gate, T, 1 if per_token else H, torch.float32 if f32 else dtype, dev)
+                kind = 2 if per_token else 3
+            params |= 4 if f32 else 0
+    else:
+        _check(post_weight is None and gate is None, "post_weight and gate belong to y")
+    return T, H, (xp, xs, yp or None, ys, gp or None, gs, kind, pre, post or None, T, H, code, params, float(residual_scale))
+
+
+def block_norm(x: torch.Tensor, pre_weight: torch.Tensor, y: Optional[torch.Tensor] = None,
+               post_weight: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+               residual_scale: float = 1.0, eps: float = 1e-6, quantize: bool = False):
+    """Joins a block's output ``y`` to the residual stream ``x`` and norms the stream for the next block::
+
+        n = y * rsqrt(mean(y^2) + eps) * post_weight      (n = y without post_weight)
+        s = residual_scale * x + gate * n                 (s = x without y, whatever the scale)
+        h = s * rsqrt(mean(s^2) + eps) * pre_weight
+
+    x, y: float32 / bfloat16 / float16 [T, H], rows may lie apart; weights [H] and ``gate`` -- [H] per channel, [T, 1]
+    per token or [T, H] -- in the same type or float32.  Returns (s, h, rstd): s is ``x`` itself without y, rstd float32
+    [T, 2] is what ``block_norm_backward`` takes.  With ``quantize`` h is the pair (e4m3 [T, H], float32 scales
+    [H / 128, T]) that ``run`` takes as hidden_states and hidden_states_scale, rounded from the unrounded h; H must then
+    be a multiple of 128 and all rows 16-byte aligned.  Arithmetic is float32, what is stored is rounded once."""
+    T, H, args = _norm_inputs(x, pre_weight, y, post_weight, gate, residual_scale)
+    _check(eps > 0.0, "eps must be positive")
+    if quantize:
+        _check(H % BLOCK == 0, f"quantize needs a multiple of {BLOCK} columns")
+        per_token = gate is not None and gate.dim() == 2 and gate.shape[1] == 1
+        _check(_aligned(x) and _aligned(y) and _aligned(pre_weight) and _aligned(post_weight) and
+               (per_token or _aligned(gate)), "quantize needs rows that are 16-byte aligned")
+    _on_gpu(x)
+    dev = x.device
+    s = x if y is None else torch.empty((T, H), dtype=x.dtype, device=dev)
+    rstd = torch.empty((T, 2), dtype=torch.float32, device=dev)
+    scale = None
+    if quantize:
+        h = torch.empty((T, H), dtype=torch.float8_e4m3fn, device=dev)
+        scale = torch.empty((H // BLOCK, T), dtype=torch.float32, device=dev)
+    else:
+        h = torch.empty((T, H), dtype=x.dtype, device=dev)
+    if T:
+        with _on_device(dev):
+            rc = loader.lib.moe_fp8_block_scale_block_norm(
+                *args, eps, None if y is None else s.data_ptr(), h.data_ptr(), scale.data_ptr() if quantize else None,
+                rstd.data_ptr(), _stream_of(dev))
+        if rc:
+            loader.check(rc)
+    return s, ((h, scale) if quantize else h), rstd
+
+
+def block_norm_backward(x: torch.Tensor, pre_weight: torch.Tensor, rstd: torch.Tensor, grad_h: torch.Tensor,
+                        grad_stream: Optional[torch.Tensor] = None, y: Optional[torch.Tensor] = None,
+                        post_weight: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                        residual_scale: float = 1.0) -> Dict[str, Optional[torch.Tensor]]:
+    """Gradients of ``block_norm`` with the same x, y, weights, gate and scale and the ``rstd`` it returned.  grad_h [T, H]
+    belongs to h (straight through the quantisation), grad_stream [T, H] to s (None: zero).  Returns a dict with the
+    gradients of ``x``, ``y``, ``gate``, ``pre_weight`` and ``post_weight`` in their shapes and types, None where there
+    is no such argument.  Sums over tokens are float32 in a fixed order."""
+    T, H, args = _norm_inputs(x, pre_weight, y, post_weight, gate, residual_scale)
+    dev, dtype = x.device, x.dtype
+    _check(rstd.dtype == torch.float32 and tuple(rstd.shape) == (T, 2) and rstd.is_contiguous() and rstd.device == dev,
+           "rstd must be the float32 [T, 2] that block_norm returned")
+    gh = _rows("grad_h", grad_h, T, H, dtype, dev)
+    gs = (None, 0) if grad_stream is None else _rows("grad_stream", grad_stream, T, H, dtype, dev)
+    _on_gpu(x)
+    new = torch.empty if T else torch.zeros        # no token: the sums over tokens are zero
+    out = {"x": torch.empty((T, H), dtype=dtype, device=dev),
+           "pre_weight": new(H, dtype=pre_weight.dtype, device=dev),
+           "y": None if y is None else torch.empty((T, H), dtype=dtype, device=dev),
+           "post_weight": None if post_weight is None else new(H, dtype=post_weight.dtype, device=dev),
+           "gate": None if gate is None else new(gate.shape, dtype=gate.dtype, device=dev)}
+    if T:
+        ws = _scratch("norm", loader.lib.moe_fp8_block_scale_block_norm_backward_workspace_bytes, T, H, dev)
+        ptr = {k: None if v is None else v.data_ptr() for k, v in out.items()}
+        with _on_device(dev):
+            rc = loader.lib.moe_fp8_block_scale_block_norm_backward(
+                *args, rstd.data_ptr(), *gh, *gs, ptr["x"], ptr["y"], ptr["gate"], ptr["pre_weight"],
+                ptr["post_weight"], ws.data_ptr(), ws.numel(), _stream_of(dev))
+        if rc:
+            loader.check(rc)
+    return out
+
+
+def _balance_inputs(logits, top_k, cu_seqlens, token_mask, scoring):
+    """Checks what both directions of the balance loss take; returns (type code, T, E, S, arguments after K)."""
+    code = _TYPE_CODE.get(logits.dtype)
+    _check(code is not None and logits.dim() == 2, "logits must be float32, bfloat16 or float16 [T, E]")
+    T, E = logits.shape
+    dev = logits.device
+    _check(1 <= E <= BALANCE_MAX_EXPERTS and T < 2 ** 31, f"logits must have 1 to {BALANCE_MAX_EXPERTS} columns")
+    _check(E == 1 or logits.stride(1) == 1, "logits: the elements of a row must be adjacent")
+    _check(1 <= top_k <= E, "every token selects 1 to E experts")
+    _check(scoring in _SCORING, "scoring must be 'sigmoid' or 'softmax'")
+    S, cu = 1, None
+    if cu_seqlens is not None:
+        _check(cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1 and
+               cu_seqlens.is_contiguous() and cu_seqlens.device == dev, f"cu_seqlens must be int32 [sequences + 1] on {dev}")
+        S, cu = cu_seqlens.shape[0] - 1, cu_seqlens.data_ptr()
+    mask = None
+    if token_mask is not None:
+        _check(token_mask.dtype == torch.bool and tuple(token_mask.shape) == (T,) and token_mask.is_contiguous() and
+               token_mask.device == dev, f"token_mask must be bool [{T}] on {dev}")
+        mask = token_mask.data_ptr() or None
+    return code, T, E, S, (cu, S, mask, _SCORING[scoring])
+
+
+def balance_loss(logits: torch.Tensor, topk_idx: torch.Tensor, alpha: float, cu_seqlens: Optional[torch.Tensor] = None,
+                 token_mask: Optional[torch.Tensor] = None, scoring: str = "sigmoid"):
+    """Balance loss of a routing, per sequence, with the per-expert counts::
+
+        p = s / sum(s),  s = sigmoid(logits) or exp(logits)        ("sigmoid": the routing of ``route``)
+        loss[q] = alpha * sum_i f_i P_i,  f_i = E / (K n) counts[q, i],  P_i = mean of p[:, i] over the n tokens
+
+    logits float32 / bfloat16 / float16 [T, E]; topk_idx int32 [T, K], what ``route`` returns (indices outside [0, E)
+    count nowhere).  cu_seqlens int32 [S + 1] has the ascending borders of packed sequences (tokens outside every
+    sequence are left out; None: one sequence); tokens with a False in token_mask [T] are left out too, whatever their
+    rows hold.  Returns (loss float32 [S], counts int32 [S, E], tokens int32 [S]); a sequence without a token has loss 0."""
+    _check(topk_idx.dtype == torch.int32 and topk_idx.dim() == 2 and topk_idx.is_contiguous() and
+           topk_idx.device == logits.device, "topk_idx must be a contiguous int32 [T, K] on the logits' device")
+    code, T, E, S, rest = _balance_inputs(logits, topk_idx.shape[1], cu_seqlens, token_mask, scoring)
+    _check(topk_idx.shape[0] == T, "topk_idx must have a row for every token")
+    _on_gpu(logits)
+    dev = logits.device
+    loss = torch.empty(S, dtype=torch.float32, device=dev)
+    counts = torch.empty((S, E), dtype=torch.int32, device=dev)
+    tokens = torch.empty(S, dtype=torch.int32, device=dev)
+    if S:
+        ws = _scratch("balance", loader.lib.moe_fp8_block_scale_balance_loss_workspace_bytes, T, E, dev)
+        with _on_device(dev):
+            rc = loader.lib.moe_fp8_block_scale_balance_loss(
+                logits.data_ptr(), logits.stride(0), code, topk_idx.data_ptr(), T, E, topk_idx.shape[1], *rest, float(alpha),
+                loss.data_ptr(), counts.data_ptr(), tokens.data_ptr(), ws.data_ptr(), ws.numel(), _stream_of(dev))
+        if rc:
+            loader.check(rc)
+    return loss, counts, tokens
+
+
+def balance_loss_backward(grad_loss: torch.Tensor, logits: torch.Tensor, counts: torch.Tensor, tokens: torch.Tensor,
+                          top_k: int, alpha: float, cu_seqlens: Optional[torch.Tensor] = None,
+                          token_mask: Optional[torch.Tensor] = None, scoring: str = "sigmoid") -> torch.Tensor:
+    """Gradient of ``balance_loss`` for the logits, in their type, given the gradient of its losses (float32 [S]) and the
+    counts and tokens it returned; the counts are constants.  Rows of tokens that were left out are zero."""
+    code, T, E, S, rest = _balance_inputs(logits, top_k, cu_seqlens, token_mask, scoring)
+    dev = logits.device
+    _check(grad_loss.dtype == torch.float32 and tuple(grad_loss.shape) == (S,) and grad_loss.is_contiguous() and
+           grad_loss.device == dev, f"grad_loss must be a contiguous float32 [{S}] on {dev}")
+    _check(counts.dtype == torch.int32 and tuple(counts.shape) == (S, E) and counts.is_contiguous() and
+           counts.device == dev, f"counts must be a contiguous int32 [{S}, {E}] on {dev}")
+    _check(tokens.dtype == torch.int32 and tuple(tokens.shape) == (S,) and tokens.is_contiguous() and
+           tokens.device == dev, f"tokens must be a contiguous int32 [{S}] on {dev}")
+    _on_gpu(logits)
+    grad = torch.empty((T, E), dtype=logits.dtype, device=dev)
+    if T:
+        with _on_device(dev):
+            rc = loader.lib.moe_fp8_block_scale_balance_loss_backward(
+                grad_loss.data_ptr(), logits.data_ptr(), logits.stride(0), code, counts.data_ptr(), tokens.data_ptr(),
+                T, E, top_k, *rest, float(alpha), grad.data_ptr(), _stream_of(dev))
+        if rc:
+            loader.check(rc)
+    return grad
+
+
+def matvec_w4(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor] = None,
+              experts: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """Products of a decode-sized batch with 4-bit weights and group scales::
+
+        out[r, n] = sum_k x[r, k] * (q[n, k] - zero[n, k // G]) * scale[n, k // G]
+
+    x bfloat16 / float16 [R, K]; qweight uint8 [N, K / 2], two values a byte, the even k in the low half; scale
+    [N, K / G] in x's type or float32, G = 32, 64 or 128; zero uint8 [N, K / G] (None: 8).  With ``experts`` the weights
+    have a leading dimension E and every (row, choice) has its own matrix: experts int32 [R] gives out [R, N], [R, k]
+    gives [R, k, N] (the experts that ``route`` selected, less the shard's first); an expert outside [0, E) gives zeros.
+    At most 256 (row, choice) pairs.  out has x's type, or float32 with ``out_dtype``; sums are float32."""
+    code = _TYPE_CODE.get(x.dtype) if x.dtype != torch.float32 else None
+    _check(code is not None and x.dim() == 2, "x must be bfloat16 or float16 [R, K]")
+    R, K = x.shape
+    dev = x.device
+    lead = 0 if experts is None else 1
+    _check(qweight.dtype == torch.uint8 and qweight.dim() == 2 + lead and qweight.is_contiguous() and
+           qweight.device == dev and K >= 1 and qweight.shape[-1] * 2 == K and qweight.numel() > 0,
+           f"qweight must be a contiguous uint8 [{'E, ' if lead else ''}N, {K} / 2] on {dev}")
+    E, N = (qweight.shape[0] if lead else 1), qweight.shape[-2]
+    groups = scale.shape[-1] if scale.dim() else 0
+    G = K // groups if groups else 0
+    _check(G in (32, 64, 128) and G * groups == K and (scale.dtype == x.dtype or scale.dtype == torch.float32) and
+           scale.shape[:-1] == qweight.shape[:-1] and scale.is_contiguous() and scale.device == dev,
+           f"scale must be a contiguous {x.dtype} or float32 [{'E, ' if lead else ''}N, K / G] on {dev}, G = 32, 64 or 128")
+    _check(zero is None or (zero.dtype == torch.uint8 and zero.shape == scale.shape and zero.is_contiguous() and
+                            zero.device == dev), "zero must be a contiguous uint8 tensor of scale's shape")
+    stride = x.stride()
+    _check((K == 1 or stride[1] == 1) and (R <= 1 or stride[0] % 8 == 0) and x.data_ptr() % 16 == 0,
+           "the rows of x must be 16-byte aligned and their elements adjacent")
+    per_row, shape, ids = 1, (R, N), None
+    if lead:
+        _check(experts.dtype == torch.int32 and experts.dim() in (1, 2) and experts.shape[0] == R and
+               experts.is_contiguous() and experts.device == dev, f"experts must be a contiguous int32 [{R}] or [{R}, k] on {dev}")
+        per_row = experts.shape[1] if experts.dim() == 2 else 1
+        shape, ids = tuple(experts.shape) + (N,), experts.data_ptr()
+    _check(R * per_row <= MATVEC_MAX_PAIRS, f"at most {MATVEC_MAX_PAIRS} (row, expert) pairs")
+    _check(out_dtype is None or out_dtype == x.dtype or out_dtype == torch.float32, "out_dtype must be x's type or float32")
+    _on_gpu(x)
+    out = torch.empty(shape, dtype=out_dtype or x.dtype, device=dev)
+    if R * per_row:
+        with _on_device(dev):
+            rc = loader.lib.moe_fp8_block_scale_matvec_w4(
+                x.data_ptr(), stride[0], code, qweight.data_ptr(), scale.data_ptr(), scale.dtype == torch.float32,
+                None if zero is None else zero.data_ptr(), ids, R * per_row, per_row, E, N, K, G, out.data_ptr(),
+                out.dtype == torch.float32, _stream_of(dev))
+        if rc:
+            loader.check(rc)
+    return out
+
+
 def kernel_status(workspace: Optional[Workspace] = None, device=None) -> int:
     """Waits for the current stream and returns the kernels' error bits (0 = none)."""
     dev = torch.device(device if device is not None else "cuda")
