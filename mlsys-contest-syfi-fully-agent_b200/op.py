@@ -248,7 +248,7 @@ def quantize_activations(hidden_bf16: torch.Tensor):
 
 _TYPE_CODE = {torch.float32: loader.F32, torch.bfloat16: loader.BF16, torch.float16: loader.F16}
 _SCORING = {"sigmoid": loader.SCORE_SIGMOID, "softmax": loader.SCORE_SOFTMAX}
-NORM_MAX_WIDTH, BALANCE_MAX_EXPERTS, MATVEC_MAX_PAIRS = 16384, 1024, 256
+NORM_MAX_WIDTH, BALANCE_MAX_EXPERTS, MATVEC_MAX_PAIRS, MATVEC_MAX_EXPERTS = 16384, 1024, 256, 1024
 _scratch_bytes: Dict[tuple, int] = {}          # library's workspace size per kind and sizes
 
 
@@ -481,7 +481,7 @@ def matvec_w4(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor, zero:
     [N, K / G] in x's type or float32, G = 32, 64 or 128; zero uint8 [N, K / G] (None: 8).  With ``experts`` the weights
     have a leading dimension E and every (row, choice) has its own matrix: experts int32 [R] gives out [R, N], [R, k]
     gives [R, k, N] (the experts that ``route`` selected, less the shard's first); an expert outside [0, E) gives zeros.
-    At most 256 (row, choice) pairs.  out has x's type, or float32 with ``out_dtype``; sums are float32."""
+    At most 256 (row, choice) pairs and 1024 experts.  out has x's type, or float32 with ``out_dtype``; sums are float32."""
     code = _TYPE_CODE.get(x.dtype) if x.dtype != torch.float32 else None
     _check(code is not None and x.dim() == 2, "x must be bfloat16 or float16 [R, K]")
     R, K = x.shape
@@ -503,6 +503,7 @@ def matvec_w4(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor, zero:
            "the rows of x must be 16-byte aligned and their elements adjacent")
     per_row, shape, ids = 1, (R, N), None
     if lead:
+        _check(E <= MATVEC_MAX_EXPERTS, f"at most {MATVEC_MAX_EXPERTS} experts")
         _check(experts.dtype == torch.int32 and experts.dim() in (1, 2) and experts.shape[0] == R and
                experts.is_contiguous() and experts.device == dev, f"experts must be a contiguous int32 [{R}] or [{R}, k] on {dev}")
         per_row = experts.shape[1] if experts.dim() == 2 else 1
