@@ -319,7 +319,7 @@ int moe_fp8_block_scale_balance_loss_backward(const float* grad_loss, const void
  *   out[p, n] = sum_k x[p / pairs_per_row, k] * (q[e, n, k] - z[e, n, k / G]) * scale[e, n, k / G],   e = experts[p]
  *   x [pairs / pairs_per_row, K], bf16 or fp16, rows 16-byte aligned; qweight u8 [E, N, K / 2]: two values a byte, the
  *   even k in the low half, 16-byte aligned; scale [E, N, K / G] in x's type or fp32 (scale_f32); zero u8 [E, N, K / G]
- *   with values 0..15, or NULL: 8; G 32, 64 or 128, K a multiple of G
+ *   with values 0..15, or NULL: 8; G 32, 64 or 128, K <= 2^20 a multiple of G; N <= 2^22
  *   experts i32 [pairs], E <= 1024: an expert outside [0, E) is not held here, its row of out is zero; NULL with E == 1 and
  *   pairs_per_row == 1: one matrix for all rows
  *   out [pairs, N] in x's type or fp32 (out_f32).  Sums are fp32; a weight's q - z is exact. */

@@ -3,30 +3,40 @@
 // q: two values a byte, the even k in the low half; z: 8 without a table.  Pair r = (token, choice) reads row r / per_row
 // of x and expert experts[r]; a pair whose expert is not held here gives a zero row.
 //
-// Bound by the weights, which are read once per (expert, up to 8 or 16 rows).  The products run on mma.sync m16n8k16 with
-// the weights as the 16-row operand, which a lane builds in registers from the bytes it loaded itself: such an operand
-// never passes through shared memory or tensor memory, and with at most 16 columns per weight the tensor pipe is idle
-// most of the time anyway.  A lane's 16 (8, 4) bytes of a group of 128 (64, 32) weights feed eight (four, two) products in
-// whatever order of k suits the unpacking; x is staged in shared memory in that same order.  q - z is exact in the
-// activations' type (the bits of 128 + q or 1024 + q minus 128 + z or 1024 + z), products and sums are fp32, and the
-// scale multiplies the fp32 sum of its group.
+// Bound by the weights, which are read once per (expert, up to 8 or 16 rows), and next by the instructions that unpack
+// them.  The products run on mma.sync m16n8k16 with the weights as the 16-row operand, which a lane builds in registers
+// from the bytes it loaded itself: such an operand never passes through shared memory or tensor memory, and with at most
+// 16 columns per weight the tensor pipe is idle most of the time anyway.  A lane's 16 (8, 4) bytes of a group of 128 (64,
+// 32) weights feed eight (four, two) products in whatever order of k suits the unpacking; x is staged in shared memory in
+// that same order.
 //
-// A CTA owns 64 weight rows and a slice of K; its warps split rows and K, the CTAs of a cluster split K, and the partial
-// sums meet in shared memory in a fixed order.
-#include <cooperative_groups.h>
+// Unpacking is one AND per pair: a floating-point format's codes are linear up to twice its smallest normal number, so a
+// half word with only a 4-bit field set is q or 16 q times the smallest subnormal (2^-24 in fp16, 2^-133 in bf16), which
+// the tensor cores multiply exactly.  The fields at bit 0 and at bit 4 go to accumulators of their own.  bf16 activations
+// are staged times 2^64 so that the products are normal fp32 numbers (|x| < 2^63; below 2^-57 they keep an absolute 2^-80).
+// Products and sums are fp32; per group:  sum (q - z) x = sum q x - z sum x, with sum x from the staging, and the scale
+// multiplies the fp32 result.
+//
+// One persistent CTA per SM takes a contiguous run of items (expert and up to 8 or 16 of its rows, 16 weight rows), stages
+// the rows of x that the expert has, and its sixteen warps stream weights through rings of their own (cp.async, two
+// stages of 16 rows x 256 columns a warp, 64 KB in flight per SM), which run on across items.  A warp has an item to
+// itself, or several warps share its K when there are too few items; then their sums meet in shared memory in a fixed
+// order.
+#include <limits.h>
 
 #include "elem_device.cuh"
 
 namespace moe {
 namespace {
 
-namespace cg = cooperative_groups;
-
 constexpr int kMaxPairs = 256;
 constexpr int kMaxMatvecExperts = 1024;
-constexpr int kThreads = 256;
-constexpr int kTileRows = 64;
-constexpr int kSliceK = 2048;              // columns of x staged at a time
+constexpr int kWarps = 16;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kDepth = 2;                  // stages of a warp's ring
+constexpr int kStep = 256;                 // columns of a stage
+constexpr int kTile = 16;                  // weight rows of an item
+constexpr int kSmemMost = 227 * 1024;
 
 struct MatvecArgs {
   const void* x;
@@ -35,291 +45,459 @@ struct MatvecArgs {
   const void* scale;         // [E, N, K / G]
   const uint8_t* zero;       // [E, N, K / G] or null
   const int* experts;        // [pairs] or null
-  int pairs, per_row, E, N, K, scale_f32;
-  int split;                 // CTAs of a cluster, which divide K
-  int slice_units;           // groups staged at a time
+  int pairs, per_row, E, N, K, scale_f32, out_f32;
+  int x_cols;                // rows of x that are staged at most
+  int slice_steps;           // steps of 256 columns staged at a time
   int x_row;                 // 16-byte chunks between staged rows
   void* out;                 // [pairs, N]
 };
 
-template <typename T> struct Nibble;
-template <> struct Nibble<__nv_bfloat16> {
-  static constexpr uint32_t kMagic = 0x43004300u;      // 128 + q in both halves
-  static __device__ __forceinline__ uint32_t minus(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
+template <typename T> struct Mma;
+template <> struct Mma<__nv_bfloat16> {
+  static constexpr float kUnit = 0x1p69f;              // undoes 2^-133 of the codes and 2^64 of x
+  static __device__ __forceinline__ uint32_t staged(uint32_t v) {
+    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v), __floats2bfloat162_rn(0x1p64f, 0x1p64f));
+    return *reinterpret_cast<const uint32_t*>(&r);
   }
-  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  static __device__ __forceinline__ float2 widen(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); }
+  static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 };
-template <> struct Nibble<__half> {
-  static constexpr uint32_t kMagic = 0x64006400u;      // 1024 + q
-  static __device__ __forceinline__ uint32_t minus(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-  }
-  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+template <> struct Mma<__half> {
+  static constexpr float kUnit = 0x1p24f;
+  static __device__ __forceinline__ uint32_t staged(uint32_t v) { return v; }
+  static __device__ __forceinline__ float2 widen(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+  static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 };
 
-// W consecutive words of eight weights each.
-template <int W> struct Words;
+template <int W> struct Words;             // W words of eight weights
 template <> struct Words<4> { using Type = uint4; };
 template <> struct Words<2> { using Type = uint2; };
 template <> struct Words<1> { using Type = uint32_t; };
 
-// G: group size.  NT: token tiles of eight columns.  A warp has MT tiles of 16 weight rows.
-template <typename T, typename O, int G, int NT>
-__global__ void __launch_bounds__(kThreads, 2) matvec_w4_kernel(MatvecArgs a) {
-  constexpr int MT = NT, WR = kTileRows / (16 * MT), WK = kThreads / 32 / WR;   // row groups and K parts of the warps
-  constexpr int W = G / 32;                        // words a lane loads per row and group
-  constexpr int U = (MT == 1 ? 4 : 2) * (4 / W > 2 ? 2 : 4 / W);   // groups in flight
-  constexpr int kCols = 8 * NT, kRedRow = kTileRows + 4;
-  extern __shared__ uint4 xs[];                    // [kCols][x_row] staged activations
-  __shared__ float red[WK][kCols][kRedRow];
-  __shared__ int first_of[kMaxMatvecExperts];
-  __shared__ int list[kMaxPairs], warp_count[8], chosen, n_list;
+__device__ __forceinline__ uint32_t smem_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// A stage: 16 rows of 128 bytes of weights (16-byte chunks swizzled by row, so that 4-, 8- and 16-byte reads of eight rows
+// are free of bank conflicts), then per row the aligned words that hold its scales, then those with its zero points.
+template <int G, bool ZERO> struct Stage {
+  static constexpr int kGroups = kStep / G;
+  static constexpr int kScaleWords = kGroups;                        // fp32: one each; 16 bits: kGroups / 2 + 1 at most
+  static constexpr int kZeroWords = ZERO ? (kGroups + 6) / 4 : 0;
+  static constexpr int kScales = kTile * kStep / 2, kZeros = kScales + kTile * 4 * kScaleWords;
+  static constexpr int kBytes = kZeros + kTile * 4 * kZeroWords;
+};
+__device__ __forceinline__ int swizzle(int row) { return (row & 1) << 2 | (row & 2) | ((row >> 2) & 1); }
+
+// The batch by experts: rows that chose the same expert, in batches of a column tile.
+struct Jobs {
+  int list[kMaxPairs];       // pairs, by expert in order of first appearance, ascending inside
+  int expert[kMaxPairs], first[kMaxPairs], cols[kMaxPairs];   // of a job: its expert, first entry of list, entries
+  int n;
+};
+
+// Fills `jobs` from experts[]; every CTA does it for itself (a few hundred cycles).  `table` has an entry per expert.
+__device__ __forceinline__ void find_jobs(const MatvecArgs& a, int max_cols, Jobs& jobs, int* table, int* scan) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int e = -1;
+  if (tid < a.pairs) e = a.experts ? a.experts[tid] : 0;
+  const bool held = e >= 0 && e < a.E;
+  if (held) table[e] = 0;
+  __syncthreads();
+  // place among the pairs of the same expert: warp after warp, so that the order is the pairs' own
+  const uint32_t peers = __match_any_sync(0xFFFFFFFFu, held ? e : -1);
+  const int below = __popc(peers & ((1u << lane) - 1));
+  int place = 0;
+  for (int w = 0; w < (a.pairs + 31) / 32; ++w) {
+    if (warp == w && held) place = table[e] + below;
+    __syncthreads();
+    if (warp == w && held && below == 0) table[e] += __popc(peers);
+    __syncthreads();
+  }
+  // the first pair of an expert opens its jobs; entries and jobs before them by a scan over the CTA, both in one word
+  const int count = held && place == 0 ? table[e] : 0;
+  const int opened = (count + max_cols - 1) / max_cols;
+  int before = count | opened << 16;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xFFFFFFFFu, before, d);
+    if (lane >= d) before += o;
+  }
+  if (lane == 31) scan[warp] = before;
+  __syncthreads();
+  before -= count | opened << 16;
+  for (int w = 0; w < warp; ++w) before += scan[w];
+  if (tid == kThreads - 1) jobs.n = (before >> 16) + opened;
+  if (count) {
+    const int first = before & 0xFFFF;
+    table[e] = first;
+    for (int j = 0; j < opened; ++j) {
+      const int at = (before >> 16) + j;
+      jobs.expert[at] = e;
+      jobs.first[at] = first + j * max_cols;
+      jobs.cols[at] = min(max_cols, count - j * max_cols);
+    }
+  }
+  __syncthreads();
+  if (held) jobs.list[table[e] + place] = tid;
+  __syncthreads();
+}
+
+template <typename T>
+__device__ __forceinline__ void store_result(const MatvecArgs& a, int pair, int n, float v) {
+  const int64_t at = static_cast<int64_t>(pair) * a.N + n;
+  if (a.out_f32) static_cast<float*>(a.out)[at] = v;
+  else static_cast<T*>(a.out)[at] = from_f32<T>(v);
+}
+
+// sum += the products of a stage: 16 rows and 256 columns with USED of NT column tiles.
+template <typename T, int G, int USED, int NT, bool ZERO>
+__device__ __forceinline__ void step(const MatvecArgs& a, const uint8_t* stage, const uint8_t* const (&x_at)[NT], const float* xs_at,
+                                     int u, const int (&s_low)[2], const int (&z_low)[2], int gid, int quad, float (&sum)[NT][4]) {
+  using S = Stage<G, ZERO>;
+  constexpr int W = G / 32;                        // words of a lane per row and group
+#pragma unroll
+  for (int gi = 0; gi < S::kGroups; ++gi) {
+    typename Words<W>::Type w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // the lane's W words of the group: byte gi * G / 2 + quad * 4 W of the row
+      const int r = gid + 8 * h, byte = gi * (G / 2) + quad * (4 * W);
+      w[h] = *reinterpret_cast<const typename Words<W>::Type*>(stage + r * (kStep / 2) + ((byte >> 4) ^ swizzle(r)) * 16 + (byte & 15));
+    }
+    float even[USED][4] = {}, odd[USED][4] = {};   // sums over the fields at bit 0 and at bit 4 of a byte
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const uint32_t lo = reinterpret_cast<const uint32_t*>(&w[0])[j];
+      const uint32_t hi = reinterpret_cast<const uint32_t*>(&w[1])[j];
+      const uint32_t fe[4] = {lo & 0x000F000Fu, hi & 0x000F000Fu, (lo >> 8) & 0x000F000Fu, (hi >> 8) & 0x000F000Fu};
+      const uint32_t fo[4] = {lo & 0x00F000F0u, hi & 0x00F000F0u, (lo >> 8) & 0x00F000F0u, (hi >> 8) & 0x00F000F0u};
+#pragma unroll
+      for (int t = 0; t < USED; ++t) {
+        const uint4 b = *reinterpret_cast<const uint4*>(x_at[t] + gi * (2 * G) + 64 * j);
+        Mma<T>::run(even[t], fe, b.x, b.y);
+        Mma<T>::run(odd[t], fo, b.z, b.w);
+      }
+    }
+    float2 xt[USED];
+#pragma unroll
+    for (int t = 0; t < USED; ++t) xt[t] = *reinterpret_cast<const float2*>(xs_at + gi * (8 * NT) + 8 * t);
+    const bool there = gi == 0 || u * kStep + gi * G < a.K;            // groups behind K have zeros for x and q
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = gid + 8 * h;
+      const uint8_t* s_at = stage + S::kScales + r * 4 * S::kScaleWords;
+      float scale;
+      if (a.scale_f32)
+        scale = *reinterpret_cast<const float*>(s_at + gi * 4);
+      else
+        scale = to_f32<T>(*reinterpret_cast<const T*>(s_at + ((s_low[h] + u * (S::kGroups * 2)) & 2) + gi * 2));
+      if (!there) scale = 0.0f;
+      float zero = 8.0f;
+      if (ZERO) zero = static_cast<float>(stage[S::kZeros + r * 4 * S::kZeroWords + ((z_low[h] + u * S::kGroups) & 3) + gi]);
+      const float unit = scale * Mma<T>::kUnit;
+      zero *= scale;
+#pragma unroll
+      for (int t = 0; t < USED; ++t) {
+        sum[t][2 * h] += (even[t][2 * h] + 0.0625f * odd[t][2 * h]) * unit - zero * xt[t].x;
+        sum[t][2 * h + 1] += (even[t][2 * h + 1] + 0.0625f * odd[t][2 * h + 1]) * unit - zero * xt[t].y;
+      }
+    }
+  }
+}
+
+// Where a warp is in its sequence of (job, round, slice, step).
+struct Cursor {
+  int job, round, slice, u, end;
+  int tile, tile_end;        // first tile of the CTA's run in this job and the one behind its last
+  int wk;                    // warps that share an item of the run
+};
+
+// G: group size.  NT: token tiles of eight columns.  ZERO: a table of zero points.
+template <typename T, int G, int NT, bool ZERO>
+__global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
+  using S = Stage<G, ZERO>;
+  constexpr int W = G / 32, kCols = 8 * NT;
+  extern __shared__ __align__(16) uint8_t smem[];  // rings of the warps, staged x, a group of zeros, sums of x
+  __shared__ float red[2][kWarps][kCols][kTile + 4];
+  __shared__ Jobs jobs;
+  __shared__ int scan[kWarps];
+  static_assert(sizeof(red) >= kMaxMatvecExperts * sizeof(int), "find_jobs' table lies in red");
   griddep_launch_dependents();
   griddep_wait();
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, quad = lane & 3;
-  const int rank = blockIdx.x % a.split, n0 = blockIdx.x / a.split * kTileRows;
-  O* out = static_cast<O*>(a.out);
-
-  // Slot y works for the y-th different expert of the batch, in order of first appearance, on all rows that chose it.
-  int expert = 0, pairs = a.pairs;
+  uint4* const xs = reinterpret_cast<uint4*>(smem + kWarps * kDepth * S::kBytes);
+  uint4* const none = xs + a.x_cols * a.x_row;     // what lanes without a column multiply
+  float* const xsum = reinterpret_cast<float*>(none + kStep / 8);   // [groups of a slice][kCols]
+  const uint32_t ring = smem_address(smem) + warp * kDepth * S::kBytes;
+  if (tid < kStep / 8) none[tid] = make_uint4(0u, 0u, 0u, 0u);
+  find_jobs(a, kCols, jobs, reinterpret_cast<int*>(red), scan);
   if (a.experts) {
-    const int e = tid < a.pairs ? a.experts[tid] : -1;
-    const bool held = e >= 0 && e < a.E;
-    if (tid == 0) chosen = -1;
-    if (held) first_of[e] = kMaxPairs;
-    __syncthreads();
-    if (held) atomicMin(first_of + e, tid);
-    __syncthreads();
-    const bool first = held && first_of[e] == tid;
-    const uint32_t firsts = __ballot_sync(0xFFFFFFFFu, first);
-    if (lane == 0) warp_count[warp] = __popc(firsts);
-    __syncthreads();
-    int before = __popc(firsts & ((1u << lane) - 1));
-    for (int w = 0; w < warp; ++w) before += warp_count[w];
-    if (first && before == blockIdx.y) chosen = e;
-    if (rank == 0 && tid < a.pairs && !held && tid % gridDim.y == blockIdx.y) {
-      for (int n = n0; n < min(n0 + kTileRows, a.N); ++n) out[static_cast<int64_t>(tid) * a.N + n] = from_f32<O>(0.0f);
+    for (int p = 0; p < a.pairs; ++p) {
+      const int e = a.experts[p];
+      if (e >= 0 && e < a.E) continue;
+      for (int n = blockIdx.x * kThreads + tid; n < a.N; n += gridDim.x * kThreads) store_result<T>(a, p, n, 0.0f);
     }
-    __syncthreads();
-    expert = chosen;
-    if (expert < 0) return;                        // the same in all CTAs of a cluster
-    const uint32_t mine = __ballot_sync(0xFFFFFFFFu, held && e == expert);
-    if (lane == 0) warp_count[warp] = __popc(mine);
-    __syncthreads();
-    before = __popc(mine & ((1u << lane) - 1));
-    for (int w = 0; w < warp; ++w) before += warp_count[w];
-    if (held && e == expert) list[before] = tid;
-    if (tid == 0) {
-      int n = 0;
-      for (int w = 0; w < 8; ++w) n += warp_count[w];
-      n_list = n;
-    }
-    __syncthreads();
-    pairs = n_list;
   }
 
-  const int units = a.K / G, per_rank = (units + a.split - 1) / a.split;
-  const int first_unit = min(units, rank * per_rank), end_unit = min(units, first_unit + per_rank);
-  const int row_warp = n0 + (warp / WK) * 16 * MT + gid, part = warp % WK;
-  // addresses of the lane's rows (rows behind the last read the last one and are not stored)
-  int64_t row[MT][2];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) row[m][h] = static_cast<int64_t>(expert) * a.N + min(row_warp + 16 * m + 8 * h, a.N - 1);
+  const int steps = (a.K + kStep - 1) / kStep, groups = a.K / G, tiles = (a.N + kTile - 1) / kTile;
+  const int slices = (steps + a.slice_steps - 1) / a.slice_steps;
+  const int64_t items = static_cast<int64_t>(jobs.n) * tiles;
+  // The CTA's run of items.  A run that goes on into the next job stages x twice and ends two rounds with idle warps, so
+  // with few jobs every CTA stays in one of them; with many, equal runs matter more.
+  int item0, item1;
+  if (jobs.n * 4 <= gridDim.x) {
+    const int g = gridDim.x, job = blockIdx.x * jobs.n / g;
+    const int lo = (job * g + jobs.n - 1) / jobs.n, n = ((job + 1) * g + jobs.n - 1) / jobs.n - lo, i = blockIdx.x - lo;
+    item0 = job * tiles + static_cast<int>(static_cast<int64_t>(tiles) * i / n);
+    item1 = job * tiles + static_cast<int>(static_cast<int64_t>(tiles) * (i + 1) / n);
+  } else {
+    item0 = static_cast<int>(items * blockIdx.x / gridDim.x);
+    item1 = static_cast<int>(items * (blockIdx.x + 1) / gridDim.x);
+  }
+  if (item0 == item1) return;
+  const int last_job = (item1 - 1) / tiles;
 
-  for (int p0 = 0; p0 < pairs; p0 += kCols) {
-    const int cols = min(kCols, pairs - p0);
-    float sum[MT][NT][4];
+  auto open_job = [&](Cursor& c) {
+    c.tile = max(item0 - c.job * tiles, 0);
+    c.tile_end = min(item1 - c.job * tiles, tiles);
+    // the fewest steps until the last warp is done with the run, with about a step's time for a join
+    int best = INT_MAX;
+    for (int k = 1; k <= kWarps; k *= 2) {
+      const int cost = (c.tile_end - c.tile + kWarps / k - 1) / (kWarps / k) * ((steps + k - 1) / k + (k > 1 ? 1 : 0));
+      if (cost < best) {
+        best = cost;
+        c.wk = k;
+      }
+    }
+  };
+  auto tile_of = [&](const Cursor& c) { return c.tile + c.round * (kWarps / c.wk) + warp / c.wk; };
+  auto open = [&](Cursor& c) {                     // the warp's steps in (job, round, slice)
+    const int s0 = c.slice * a.slice_steps, s1 = min(steps, s0 + a.slice_steps), per = (s1 - s0 + c.wk - 1) / c.wk;
+    c.u = min(s1, s0 + warp % c.wk * per);
+    c.end = tile_of(c) < c.tile_end ? min(s1, c.u + per) : c.u;
+  };
+
+  // ---- loads, which run kDepth steps ahead
+  Cursor ld = {item0 / tiles, 0, 0, 0, 0, 0, 0, 1};
+  const int row8 = lane >> 3, chunk8 = lane & 7;   // a copy instruction takes four rows of 128 bytes
+  const uint8_t* ld_q[4];                          // the lane's chunk of rows row8, row8 + 4, ...
+  uintptr_t ld_s, ld_z;                            // scales and zeros of row lane % 16
+  const int scale_size = a.scale_f32 ? 4 : 2;
+  uint32_t to_q[4];                                // where the chunks go in a stage
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+  for (int i = 0; i < 4; ++i) to_q[i] = (row8 + 4 * i) * (kStep / 2) + (chunk8 ^ swizzle(row8 + 4 * i)) * 16;
+  auto rows_of = [&]() {
+    const int n = tile_of(ld) * kTile;
+    const int64_t base = static_cast<int64_t>(jobs.expert[ld.job]) * a.N;
+    // rows behind the last read the last one and are not stored
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ld_q[i] = a.q + (base + min(n + row8 + 4 * i, a.N - 1)) * (a.K / 2) + chunk8 * 16;
+    const int64_t row = (base + min(n + (lane & 15), a.N - 1)) * groups;
+    ld_s = reinterpret_cast<uintptr_t>(a.scale) + row * scale_size;
+    ld_z = reinterpret_cast<uintptr_t>(a.zero) + row;
+  };
+  auto load = [&](uint32_t stage) {
+    while (ld.u >= ld.end && ld.job <= last_job) {
+      if (++ld.slice == slices) {
+        ld.slice = 0;
+        ++ld.round;
+        if (ld.tile + ld.round * (kWarps / ld.wk) >= ld.tile_end) {
+          ld.round = 0;
+          if (++ld.job > last_job) break;
+          open_job(ld);
+        }
+      }
+      open(ld);
+      if (ld.u < ld.end) rows_of();
+    }
+    if (ld.job <= last_job) {
+      const bool there = ld.u * kStep + chunk8 * 32 < a.K;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) copy16(stage + to_q[i], ld_q[i] + ld.u * (kStep / 2), there);
+      // aligned words around the row's scales; a word behind the last needed byte is not read
+      const int r = lane & 15, n_groups = min(S::kGroups, groups - ld.u * S::kGroups);
+      const uintptr_t from = ld_s + ld.u * (S::kGroups * scale_size);
+#pragma unroll
+      for (int i = 0; i < S::kScaleWords / 2; ++i) {
+        const int word = 2 * i + (lane >> 4);
+        const uintptr_t at = (from & ~uintptr_t(3)) + 4 * word;
+        if (at < from + n_groups * scale_size)
+          copy4(stage + S::kScales + (r * S::kScaleWords + word) * 4, reinterpret_cast<const void*>(at));
+      }
+      if (ZERO) {
+        const uintptr_t z = ld_z + ld.u * S::kGroups;
+#pragma unroll
+        for (int i = 0; i < (S::kZeroWords + 1) / 2; ++i) {
+          const int word = 2 * i + (lane >> 4);
+          const uintptr_t at = (z & ~uintptr_t(3)) + 4 * word;
+          if (word < S::kZeroWords && at < z + n_groups)
+            copy4(stage + S::kZeros + (r * S::kZeroWords + word) * 4, reinterpret_cast<const void*>(at));
+        }
+      }
+      ++ld.u;
+    }
+    copies_close();
+  };
+  open_job(ld);
+  open(ld);
+  if (ld.u < ld.end) rows_of();
+#pragma unroll
+  for (int i = 0; i < kDepth; ++i) load(ring + i * S::kBytes);
+
+  // ---- products
+  int slot = 0, par = 0;
+  Cursor at = {item0 / tiles, 0, 0, 0, 0, 0, 0, 1};
+  for (; at.job <= last_job; ++at.job) {
+    open_job(at);
+    const int cols = jobs.cols[at.job], first = jobs.first[at.job], wk = at.wk, at_once = kWarps / wk;
+    for (at.round = 0; at.tile + at.round * at_once < at.tile_end; ++at.round) {
+      const int n0 = tile_of(at) * kTile;
+      float sum[NT][4];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[m][t][i] = 0.0f;
+        for (int i = 0; i < 4; ++i) sum[t][i] = 0.0f;
 
-    for (int s0 = first_unit; s0 < end_unit; s0 += a.slice_units) {
-      const int s1 = min(end_unit, s0 + a.slice_units), per_part = (s1 - s0 + WK - 1) / WK;
-      const int u0 = s0 + part * per_part, u1 = min(s1, u0 + per_part);
-      typename Words<W>::Type w[U][MT][2];
-      float sc[U][MT][2];
-      uint32_t zp[U][MT][2];
-      auto load = [&](int u) {
+      for (at.slice = 0; at.slice < slices; ++at.slice) {
+        const int s0 = at.slice * a.slice_steps, s1 = min(steps, s0 + a.slice_steps);
+        if (at.round == 0 || slices > 1) {
+          // stage x: a 16-byte chunk holds eight k, stored as the pairs (0, 4), (2, 6), (1, 5), (3, 7); chunk j of quad
+          // lane t of a group lies at 4 j + t
+          __syncthreads();
+          const int chunks = (s1 - s0) * (kStep / 8), held = (min(a.K, s1 * kStep) - s0 * kStep) / 8;   // zeros behind K
+          const int blocks = chunks / 32;
+#pragma unroll 4
+          for (int b = warp; b < cols * blocks; b += kWarps) {
+            const int c = b / blocks, i = (b - c * blocks) * 32 + lane, in = i % (G / 8);
+            const T* row = static_cast<const T*>(a.x) + (jobs.list[first + c] / a.per_row) * a.x_stride + static_cast<int64_t>(s0) * kStep;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (i < held) v = __ldg(reinterpret_cast<const uint4*>(row) + i);
+            xs[c * a.x_row + i - in + (in % W) * 4 + in / W] =
+                make_uint4(Mma<T>::staged(__byte_perm(v.x, v.z, 0x5410)), Mma<T>::staged(__byte_perm(v.y, v.w, 0x5410)),
+                           Mma<T>::staged(__byte_perm(v.x, v.z, 0x7632)), Mma<T>::staged(__byte_perm(v.y, v.w, 0x7632)));
+            const float2 p = Mma<T>::widen(v.x), q = Mma<T>::widen(v.y), r = Mma<T>::widen(v.z), t = Mma<T>::widen(v.w);
+            float total = ((p.x + p.y) + (q.x + q.y)) + ((r.x + r.y) + (t.x + t.y));
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-          if (u + i >= u1) continue;
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              w[i][m][h] = __ldg(reinterpret_cast<const typename Words<W>::Type*>(a.q + row[m][h] * (a.K / 2) +
-                                                                                 (u + i) * (G / 2) + quad * (4 * W)));
-        }
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-          if (u + i >= u1) continue;
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int64_t at = row[m][h] * units + u + i;
-              sc[i][m][h] = a.scale_f32 ? __ldg(static_cast<const float*>(a.scale) + at)
-                                        : to_f32<T>(static_cast<const T*>(a.scale)[at]);
-              zp[i][m][h] = a.zero ? Nibble<T>::kMagic | __ldg(a.zero + at) * 0x00010001u : Nibble<T>::kMagic | 0x00080008u;
-            }
-        }
-      };
-      load(u0);
-
-      // stage x: a 16-byte chunk holds eight k, stored as pairs (k, k + 4); chunk j of quad lane t of a group at 4 j + t
-      const int chunks = (s1 - s0) * (G / 8);
-      for (int i = tid; i < cols * chunks; i += kThreads) {
-        const int c = i / chunks, at = i - c * chunks, in = at % (G / 8);
-        const int pair = a.experts ? list[p0 + c] : p0 + c;
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (pair / a.per_row) * a.x_stride +
-                                                             static_cast<int64_t>(s0) * G + at * 8));
-        xs[c * a.x_row + at - in + (in % W) * 4 + in / W] =
-            make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
-                       __byte_perm(v.y, v.w, 0x7632));
-      }
-      __syncthreads();
-
-      for (int u = u0; u < u1; u += U) {
-        if (u != u0) load(u);
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-          if (u + i >= u1) continue;
-          float acc[MT][NT][4];
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) acc[m][t][k] = 0.0f;
-          const uint4* xu = xs + (u + i - s0) * (G / 8) + quad;
-#pragma unroll
-          for (int j = 0; j < W; ++j) {
-            uint4 b[NT];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              b[t] = make_uint4(0u, 0u, 0u, 0u);
-              if (8 * t + gid < cols) b[t] = xu[(8 * t + gid) * a.x_row + 4 * j];
-            }
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              const uint32_t lo = reinterpret_cast<const uint32_t*>(&w[i][m][0])[j];
-              const uint32_t hi = reinterpret_cast<const uint32_t*>(&w[i][m][1])[j];
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                uint32_t frag[4];
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  const int shift = 4 * (2 * half + k);
-                  frag[2 * k] = Nibble<T>::minus(((lo >> shift) & 0x000F000Fu) | Nibble<T>::kMagic, zp[i][m][0]);
-                  frag[2 * k + 1] = Nibble<T>::minus(((hi >> shift) & 0x000F000Fu) | Nibble<T>::kMagic, zp[i][m][1]);
-                }
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                  if (t > 0 && cols <= 8 * t) continue;
-                  Nibble<T>::mma(acc[m][t], frag, half ? b[t].z : b[t].x, half ? b[t].w : b[t].y);
-                }
-              }
-            }
+            for (int d = G / 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
+            if (in == 0) xsum[i / (G / 8) * kCols + c] = total;
           }
+          __syncthreads();
+        }
+        open(at);
+        const int64_t row = static_cast<int64_t>(jobs.expert[at.job]) * a.N;
+        // low address bits of the scales and zeros of the lane's two rows: where they are in their aligned words
+        int s_low[2], z_low[2];
 #pragma unroll
-          for (int m = 0; m < MT; ++m)
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t r = static_cast<uint32_t>(row + min(n0 + gid + 8 * h, a.N - 1)) * static_cast<uint32_t>(groups);
+          s_low[h] = static_cast<int>(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.scale)) + r * scale_size);
+          z_low[h] = ZERO ? static_cast<int>(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.zero)) + r) : 0;
+        }
+        const uint8_t* x_at[NT];                   // lanes without a column stay on the zeros
+        int x_step[NT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t) {
+          const bool has = 8 * t + gid < cols;
+          x_at[t] = reinterpret_cast<const uint8_t*>((has ? xs + (8 * t + gid) * a.x_row + (at.u - s0) * (kStep / 8) : none) + quad);
+          x_step[t] = has ? 2 * kStep : 0;
+        }
+        for (; at.u < at.end; ++at.u) {
+          const uint8_t* const stage = smem + (warp * kDepth + slot) * S::kBytes;
+          copies_wait<kDepth - 1>();
+          __syncwarp();
+          const float* const xs_at = xsum + (at.u - s0) * (S::kGroups * kCols) + 2 * quad;
+          if (NT == 1 || cols <= 8) step<T, G, 1, NT, ZERO>(a, stage, x_at, xs_at, at.u, s_low, z_low, gid, quad, sum);
+          else step<T, G, NT, NT, ZERO>(a, stage, x_at, xs_at, at.u, s_low, z_low, gid, quad, sum);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) sum[m][t][k] += acc[m][t][k] * sc[i][m][k >> 1];
+          for (int t = 0; t < NT; ++t) x_at[t] += x_step[t];
+          __syncwarp();
+          load(ring + slot * S::kBytes);
+          slot = slot + 1 == kDepth ? 0 : slot + 1;
         }
       }
-      __syncthreads();                             // the staged rows may be overwritten
-    }
 
-    // join: the K parts of the warps, then the CTAs of the cluster, each in order
+      if (wk == 1) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+          for (int k = 0; k < 4; ++k) {
+            const int c = 8 * t + 2 * quad + (k & 1), n = n0 + gid + 8 * (k >> 1);
+            if (c < cols && n < a.N && tile_of(at) < at.tile_end) store_result<T>(a, jobs.list[first + c], n, sum[t][k]);
+          }
+      } else {
+        // join the parts in order; the two halves of `red` alternate, so the one barrier of a round also ends the reads
+        // of the round before
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          red[part][8 * t + 2 * quad + (k & 1)][(warp / WK) * 16 * MT + 16 * m + 8 * (k >> 1) + gid] = sum[m][t][k];
-    __syncthreads();
-    if (a.split == 1) {
-      for (int i = tid; i < cols * kTileRows; i += kThreads) {
-        const int c = i / kTileRows, r = i % kTileRows;
-        float v = 0.0f;
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int k = 0; k < WK; ++k) v += red[k][c][r];
-        const int pair = a.experts ? list[p0 + c] : p0 + c;
-        if (n0 + r < a.N) out[static_cast<int64_t>(pair) * a.N + n0 + r] = from_f32<O>(v);
+          for (int k = 0; k < 4; ++k) red[par][warp][8 * t + 2 * quad + (k & 1)][gid + 8 * (k >> 1)] = sum[t][k];
+        __syncthreads();
+        const int here = min(at_once, at.tile_end - at.tile - at.round * at_once);
+        for (int i = tid; i < here * cols * kTile; i += kThreads) {
+          const int r = i % kTile, c = i / kTile % cols, l = i / kTile / cols;
+          float v = 0.0f;
+          for (int k = 0; k < wk; ++k) v += red[par][l * wk + k][c][r];
+          const int n = (at.tile + at.round * at_once + l) * kTile + r;
+          if (n < a.N) store_result<T>(a, jobs.list[first + c], n, v);
+        }
+        par ^= 1;
       }
-      __syncthreads();
-    } else {
-      cg::cluster_group cluster = cg::this_cluster();
-      for (int i = tid; i < cols * kTileRows; i += kThreads) {
-        const int c = i / kTileRows, r = i % kTileRows;
-        float v = 0.0f;
-#pragma unroll
-        for (int k = 0; k < WK; ++k) v += red[k][c][r];
-        red[0][c][r] = v;
-      }
-      cluster.sync();
-      for (int i = tid + rank * kThreads; i < cols * kTileRows; i += kThreads * a.split) {
-        const int c = i / kTileRows, r = i % kTileRows;
-        float v = 0.0f;
-        for (int k = 0; k < a.split; ++k) v += *cluster.map_shared_rank(&red[0][c][r], k);
-        const int pair = a.experts ? list[p0 + c] : p0 + c;
-        if (n0 + r < a.N) out[static_cast<int64_t>(pair) * a.N + n0 + r] = from_f32<O>(v);
-      }
-      cluster.sync();                              // nobody reads a neighbour's sums any more
     }
   }
 }
 
-template <typename T, typename O, int G, int NT>
+template <typename T, int G, int NT, bool ZERO>
 cudaError_t launch_kernel(MatvecArgs a, cudaStream_t stream) {
-  const int units = a.K / G, tiles = (a.N + kTileRows - 1) / kTileRows;
-  const int slots = a.experts ? (a.pairs < a.E ? a.pairs : a.E) : 1;
-  // A cluster divides K so that a CTA stages its columns of x once, and further while there are fewer CTAs than SMs and
-  // a warp keeps at least one group.
-  int split = 1;
-  while (split < 8 && a.K > kSliceK * split) split *= 2;
-  while (split < 8 && tiles * slots * split < kNumSMs && units >= 2 * split * (NT == 1 ? 2 : 4)) split *= 2;
-  a.split = split;
-  const int per_rank = (units + split - 1) / split;
-  a.slice_units = per_rank < kSliceK / G ? per_rank : kSliceK / G;
-  a.x_row = (a.slice_units * (G / 8) + 7) / 8 * 8 + 4;   // rows 64 bytes apart in the banks
-  const size_t smem = static_cast<size_t>(8 * NT) * a.x_row * 16;
-  constexpr size_t kMost = static_cast<size_t>(8 * NT) * (kSliceK / 8 + 4) * 16;
-  static const cudaError_t set = cudaFuncSetAttribute(matvec_w4_kernel<T, O, G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                      static_cast<int>(kMost));
-  if (set != cudaSuccess) return set;
-  return launch_cluster(matvec_w4_kernel<T, O, G, NT>, dim3(tiles * split, slots), dim3(kThreads), split, smem, stream, a);
+  constexpr size_t kRing = static_cast<size_t>(kWarps) * kDepth * Stage<G, ZERO>::kBytes;
+  constexpr size_t kStatic = sizeof(float) * 2 * kWarps * 8 * NT * (kTile + 4) + sizeof(Jobs) + 4 * kWarps;
+  constexpr size_t kX = kSmemMost - kRing - kStatic - 1024 - kStep * 2;      // for staged x and its group sums
+  const auto kernel = matvec_w4_kernel<T, G, NT, ZERO>;
+  a.x_cols = a.pairs < 8 * NT ? a.pairs : 8 * NT;
+  const int steps = (a.K + kStep - 1) / kStep;
+  const size_t per_step = static_cast<size_t>(a.x_cols) * kStep * 2 + kStep / G * 8 * NT * 4;
+  int slice = static_cast<int>((kX - a.x_cols * 64) / per_step);
+  if (slice > steps) slice = steps;
+  a.slice_steps = slice;
+  a.x_row = slice * (kStep / 8) + 4;                 // rows 64 bytes apart in the banks
+  const size_t smem = kRing + static_cast<size_t>(a.x_cols) * a.x_row * 16 + kStep * 2 + static_cast<size_t>(slice) * (kStep / G) * 8 * NT * 4;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kRing + kX + kStep * 2));
+  if (e != cudaSuccess) return e;
+  const int64_t most = static_cast<int64_t>((a.N + kTile - 1) / kTile) * a.pairs;
+  return launch_pdl(kernel, dim3(static_cast<unsigned>(most < kNumSMs ? most : kNumSMs)), dim3(kThreads), smem, stream, a);
 }
 
-template <typename T, typename O>
+template <typename T, int NT>
+cudaError_t launch_group(const MatvecArgs& a, int G, cudaStream_t stream) {
+  if (a.zero) {
+    if (G == 128) return launch_kernel<T, 128, NT, true>(a, stream);
+    if (G == 64) return launch_kernel<T, 64, NT, true>(a, stream);
+    return launch_kernel<T, 32, NT, true>(a, stream);
+  }
+  if (G == 128) return launch_kernel<T, 128, NT, false>(a, stream);
+  if (G == 64) return launch_kernel<T, 64, NT, false>(a, stream);
+  return launch_kernel<T, 32, NT, false>(a, stream);
+}
+
+template <typename T>
 cudaError_t launch_matvec(const MatvecArgs& a, int G, cudaStream_t stream) {
   // one tile of eight columns where no expert can have more rows (a row chooses an expert once)
-  const bool one = a.pairs / a.per_row <= 8;
-  if (G == 128) return one ? launch_kernel<T, O, 128, 1>(a, stream) : launch_kernel<T, O, 128, 2>(a, stream);
-  if (G == 64) return one ? launch_kernel<T, O, 64, 1>(a, stream) : launch_kernel<T, O, 64, 2>(a, stream);
-  return one ? launch_kernel<T, O, 32, 1>(a, stream) : launch_kernel<T, O, 32, 2>(a, stream);
+  return a.pairs / a.per_row <= 8 ? launch_group<T, 1>(a, G, stream) : launch_group<T, 2>(a, G, stream);
 }
 
 }  // namespace
@@ -332,18 +510,14 @@ extern "C" int moe_fp8_block_scale_matvec_w4(const void* x, int64_t x_stride, in
                                              int pairs, int pairs_per_row, int E, int N, int K, int G, void* out,
                                              int out_f32, void* stream_v) {
   if (pairs < 0 || pairs > kMaxPairs || pairs_per_row < 1 || pairs % pairs_per_row != 0 || E < 1 || E > kMaxMatvecExperts ||
-      N < 1 || K < 1 || (G != 32 && G != 64 && G != 128) || K % G != 0 || (dtype != MOE_B200_BF16 && dtype != MOE_B200_F16) ||
+      N < 1 || N > (1 << 22) || K < 1 || K > (1 << 20) || (G != 32 && G != 64 && G != 128) || K % G != 0 || (dtype != MOE_B200_BF16 && dtype != MOE_B200_F16) ||
       (!experts && (E != 1 || pairs_per_row != 1)))
     return MOE_B200_EINVAL;
   if (pairs == 0) return MOE_B200_OK;
-  if (!x || !qweight || !scale || !out || !aligned(x, 16) || (pairs > pairs_per_row && x_stride % 8 != 0) || !aligned(qweight, 16))
+  if (!x || !qweight || !scale || !out || !aligned(scale, scale_f32 ? 4 : 2) || !aligned(x, 16) || (pairs > pairs_per_row && x_stride % 8 != 0) || !aligned(qweight, 16))
     return MOE_B200_EINVAL;
-  MatvecArgs a = {x, x_stride, qweight, scale, zero, experts, pairs, pairs_per_row, E, N, K, scale_f32, 1, 0, 0, out};
+  MatvecArgs a = {x, x_stride, qweight, scale, zero, experts, pairs, pairs_per_row, E, N, K, scale_f32, out_f32, 1, 0, 0, out};
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
-  cudaError_t e;
-  if (dtype == MOE_B200_BF16)
-    e = out_f32 ? launch_matvec<__nv_bfloat16, float>(a, G, stream) : launch_matvec<__nv_bfloat16, __nv_bfloat16>(a, G, stream);
-  else
-    e = out_f32 ? launch_matvec<__half, float>(a, G, stream) : launch_matvec<__half, __half>(a, G, stream);
+  const cudaError_t e = dtype == MOE_B200_BF16 ? launch_matvec<__nv_bfloat16>(a, G, stream) : launch_matvec<__half>(a, G, stream);
   return launch_status(e, 1);
 }

@@ -491,6 +491,7 @@ def matvec_w4(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor, zero:
            qweight.device == dev and K >= 1 and qweight.shape[-1] * 2 == K and qweight.numel() > 0,
            f"qweight must be a contiguous uint8 [{'E, ' if lead else ''}N, {K} / 2] on {dev}")
     E, N = (qweight.shape[0] if lead else 1), qweight.shape[-2]
+    _check(N <= 2 ** 22 and K <= 2 ** 20, "at most 2^22 rows and 2^20 columns")
     groups = scale.shape[-1] if scale.dim() else 0
     G = K // groups if groups else 0
     _check(G in (32, 64, 128) and G * groups == K and (scale.dtype == x.dtype or scale.dtype == torch.float32) and
