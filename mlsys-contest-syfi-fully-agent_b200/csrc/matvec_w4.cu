@@ -31,7 +31,7 @@ namespace {
 
 constexpr int kMaxPairs = 256;
 constexpr int kMaxMatvecExperts = 1024;
-constexpr int kWarps = 16;
+constexpr int kLogWarps = 4, kWarps = 1 << kLogWarps;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kDepth = 2;                  // stages of a warp's ring
 constexpr int kStep = 256;                 // columns of a stage
@@ -60,20 +60,20 @@ template <> struct Mma<__nv_bfloat16> {
     return *reinterpret_cast<const uint32_t*>(&r);
   }
   static __device__ __forceinline__ float2 widen(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); }
-  static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   }
 };
 template <> struct Mma<__half> {
   static constexpr float kUnit = 0x1p24f;
   static __device__ __forceinline__ uint32_t staged(uint32_t v) { return v; }
   static __device__ __forceinline__ float2 widen(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
-  static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   }
 };
 
@@ -164,12 +164,30 @@ __device__ __forceinline__ void store_result(const MatvecArgs& a, int pair, int 
   else static_cast<T*>(a.out)[at] = from_f32<T>(v);
 }
 
-// sum += the products of a stage: 16 rows and 256 columns with USED of NT column tiles.
+// sum += the products of a stage, 16 rows and 256 columns with USED of NT column tiles, times 1 / kUnit.
 template <typename T, int G, int USED, int NT, bool ZERO>
 __device__ __forceinline__ void step(const MatvecArgs& a, const uint8_t* stage, const uint8_t* const (&x_at)[NT], const float* xs_at,
-                                     int u, const int (&s_low)[2], const int (&z_low)[2], int gid, int quad, float (&sum)[NT][4]) {
+                                     int u, const int (&s_at)[2], const int (&z_low)[2], int gid, int quad, float (&sum)[NT][4]) {
   using S = Stage<G, ZERO>;
   constexpr int W = G / 32;                        // words of a lane per row and group
+  // the scales of the lane's two rows; groups behind K have zeros for x and q and need a finite scale
+  float scale[S::kGroups][2];
+  if (a.scale_f32) {
+#pragma unroll
+    for (int gi = 0; gi < S::kGroups; ++gi)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) scale[gi][h] = *reinterpret_cast<const float*>(stage + s_at[h] + gi * 4);
+  } else {
+#pragma unroll
+    for (int gi = 0; gi < S::kGroups; ++gi)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) scale[gi][h] = to_f32<T>(*reinterpret_cast<const T*>(stage + s_at[h] + gi * 2));
+  }
+  if ((u + 1) * kStep > a.K) {
+#pragma unroll
+    for (int gi = 1; gi < S::kGroups; ++gi)
+      if (u * kStep + gi * G >= a.K) scale[gi][0] = scale[gi][1] = 0.0f;
+  }
 #pragma unroll
   for (int gi = 0; gi < S::kGroups; ++gi) {
     typename Words<W>::Type w[2];
@@ -189,32 +207,22 @@ __device__ __forceinline__ void step(const MatvecArgs& a, const uint8_t* stage, 
 #pragma unroll
       for (int t = 0; t < USED; ++t) {
         const uint4 b = *reinterpret_cast<const uint4*>(x_at[t] + gi * (2 * G) + 64 * j);
-        Mma<T>::run(even[t], fe, b.x, b.y);
-        Mma<T>::run(odd[t], fo, b.z, b.w);
+        Mma<T>::run(even[t], fe, b.x, b.y, even[t]);
+        Mma<T>::run(odd[t], fo, b.z, b.w, odd[t]);
       }
     }
     float2 xt[USED];
 #pragma unroll
     for (int t = 0; t < USED; ++t) xt[t] = *reinterpret_cast<const float2*>(xs_at + gi * (8 * NT) + 8 * t);
-    const bool there = gi == 0 || u * kStep + gi * G < a.K;            // groups behind K have zeros for x and q
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = gid + 8 * h;
-      const uint8_t* s_at = stage + S::kScales + r * 4 * S::kScaleWords;
-      float scale;
-      if (a.scale_f32)
-        scale = *reinterpret_cast<const float*>(s_at + gi * 4);
-      else
-        scale = to_f32<T>(*reinterpret_cast<const T*>(s_at + ((s_low[h] + u * (S::kGroups * 2)) & 2) + gi * 2));
-      if (!there) scale = 0.0f;
       float zero = 8.0f;
       if (ZERO) zero = static_cast<float>(stage[S::kZeros + r * 4 * S::kZeroWords + ((z_low[h] + u * S::kGroups) & 3) + gi]);
-      const float unit = scale * Mma<T>::kUnit;
-      zero *= scale;
 #pragma unroll
       for (int t = 0; t < USED; ++t) {
-        sum[t][2 * h] += (even[t][2 * h] + 0.0625f * odd[t][2 * h]) * unit - zero * xt[t].x;
-        sum[t][2 * h + 1] += (even[t][2 * h + 1] + 0.0625f * odd[t][2 * h + 1]) * unit - zero * xt[t].y;
+        sum[t][2 * h] += (even[t][2 * h] + 0.0625f * odd[t][2 * h] - zero * xt[t].x) * scale[gi][h];
+        sum[t][2 * h + 1] += (even[t][2 * h + 1] + 0.0625f * odd[t][2 * h + 1] - zero * xt[t].y) * scale[gi][h];
       }
     }
   }
@@ -224,7 +232,7 @@ __device__ __forceinline__ void step(const MatvecArgs& a, const uint8_t* stage, 
 struct Cursor {
   int job, round, slice, u, end;
   int tile, tile_end;        // first tile of the CTA's run in this job and the one behind its last
-  int wk;                    // warps that share an item of the run
+  int lw;                    // log2 of the warps that share an item of the run
 };
 
 // G: group size.  NT: token tiles of eight columns.  ZERO: a table of zero points.
@@ -236,6 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
   __shared__ float red[2][kWarps][kCols][kTile + 4];
   __shared__ Jobs jobs;
   __shared__ int scan[kWarps];
+  __shared__ const T* x_row[kCols];
   static_assert(sizeof(red) >= kMaxMatvecExperts * sizeof(int), "find_jobs' table lies in red");
   griddep_launch_dependents();
   griddep_wait();
@@ -246,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
   float* const xsum = reinterpret_cast<float*>(none + kStep / 8);   // [groups of a slice][kCols]
   const uint32_t ring = smem_address(smem) + warp * kDepth * S::kBytes;
   if (tid < kStep / 8) none[tid] = make_uint4(0u, 0u, 0u, 0u);
-  find_jobs(a, kCols, jobs, reinterpret_cast<int*>(red), scan);
+  find_jobs(a, a.x_cols, jobs, reinterpret_cast<int*>(red), scan);
   if (a.experts) {
     for (int p = 0; p < a.pairs; ++p) {
       const int e = a.experts[p];
@@ -278,23 +287,24 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
     c.tile_end = min(item1 - c.job * tiles, tiles);
     // the fewest steps until the last warp is done with the run, with about a step's time for a join
     int best = INT_MAX;
-    for (int k = 1; k <= kWarps; k *= 2) {
-      const int cost = (c.tile_end - c.tile + kWarps / k - 1) / (kWarps / k) * ((steps + k - 1) / k + (k > 1 ? 1 : 0));
+#pragma unroll
+    for (int k = 0; k <= kLogWarps; ++k) {
+      const int cost = ((c.tile_end - c.tile + (kWarps >> k) - 1) >> (kLogWarps - k)) * (((steps + (1 << k) - 1) >> k) + (k > 0 ? 1 : 0));
       if (cost < best) {
         best = cost;
-        c.wk = k;
+        c.lw = k;
       }
     }
   };
-  auto tile_of = [&](const Cursor& c) { return c.tile + c.round * (kWarps / c.wk) + warp / c.wk; };
+  auto tile_of = [&](const Cursor& c) { return c.tile + (c.round << (kLogWarps - c.lw)) + (warp >> c.lw); };
   auto open = [&](Cursor& c) {                     // the warp's steps in (job, round, slice)
-    const int s0 = c.slice * a.slice_steps, s1 = min(steps, s0 + a.slice_steps), per = (s1 - s0 + c.wk - 1) / c.wk;
-    c.u = min(s1, s0 + warp % c.wk * per);
+    const int s0 = c.slice * a.slice_steps, s1 = min(steps, s0 + a.slice_steps), per = (s1 - s0 + (1 << c.lw) - 1) >> c.lw;
+    c.u = min(s1, s0 + (warp & ((1 << c.lw) - 1)) * per);
     c.end = tile_of(c) < c.tile_end ? min(s1, c.u + per) : c.u;
   };
 
   // ---- loads, which run kDepth steps ahead
-  Cursor ld = {item0 / tiles, 0, 0, 0, 0, 0, 0, 1};
+  Cursor ld = {item0 / tiles, 0, 0, 0, 0, 0, 0, 0};
   const int row8 = lane >> 3, chunk8 = lane & 7;   // a copy instruction takes four rows of 128 bytes
   const uint8_t* ld_q[4];                          // the lane's chunk of rows row8, row8 + 4, ...
   uintptr_t ld_s, ld_z;                            // scales and zeros of row lane % 16
@@ -317,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
       if (++ld.slice == slices) {
         ld.slice = 0;
         ++ld.round;
-        if (ld.tile + ld.round * (kWarps / ld.wk) >= ld.tile_end) {
+        if (ld.tile + (ld.round << (kLogWarps - ld.lw)) >= ld.tile_end) {
           ld.round = 0;
           if (++ld.job > last_job) break;
           open_job(ld);
@@ -332,13 +342,13 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
       for (int i = 0; i < 4; ++i) copy16(stage + to_q[i], ld_q[i] + ld.u * (kStep / 2), there);
       // aligned words around the row's scales; a word behind the last needed byte is not read
       const int r = lane & 15, n_groups = min(S::kGroups, groups - ld.u * S::kGroups);
-      const uintptr_t from = ld_s + ld.u * (S::kGroups * scale_size);
+      const int words = (static_cast<int>(ld_s & 3) + n_groups * scale_size + 3) / 4;
+      const uintptr_t from = (ld_s & ~uintptr_t(3)) + ld.u * (S::kGroups * scale_size);
 #pragma unroll
       for (int i = 0; i < S::kScaleWords / 2; ++i) {
         const int word = 2 * i + (lane >> 4);
-        const uintptr_t at = (from & ~uintptr_t(3)) + 4 * word;
-        if (at < from + n_groups * scale_size)
-          copy4(stage + S::kScales + (r * S::kScaleWords + word) * 4, reinterpret_cast<const void*>(at));
+        if (word < words)
+          copy4(stage + S::kScales + (r * S::kScaleWords + word) * 4, reinterpret_cast<const void*>(from + 4 * word));
       }
       if (ZERO) {
         const uintptr_t z = ld_z + ld.u * S::kGroups;
@@ -362,10 +372,10 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
 
   // ---- products
   int slot = 0, par = 0;
-  Cursor at = {item0 / tiles, 0, 0, 0, 0, 0, 0, 1};
+  Cursor at = {item0 / tiles, 0, 0, 0, 0, 0, 0, 0};
   for (; at.job <= last_job; ++at.job) {
     open_job(at);
-    const int cols = jobs.cols[at.job], first = jobs.first[at.job], wk = at.wk, at_once = kWarps / wk;
+    const int cols = jobs.cols[at.job], first = jobs.first[at.job], wk = 1 << at.lw, at_once = kWarps >> at.lw;
     for (at.round = 0; at.tile + at.round * at_once < at.tile_end; ++at.round) {
       const int n0 = tile_of(at) * kTile;
       float sum[NT][4];
@@ -381,32 +391,37 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
           // lane t of a group lies at 4 j + t
           __syncthreads();
           const int chunks = (s1 - s0) * (kStep / 8), held = (min(a.K, s1 * kStep) - s0 * kStep) / 8;   // zeros behind K
-          const int blocks = chunks / 32;
+          if (tid < cols)
+            x_row[tid] = static_cast<const T*>(a.x) + (jobs.list[first + tid] / a.per_row) * a.x_stride + static_cast<int64_t>(s0) * kStep;
+          __syncthreads();
+          for (int i = tid; i < chunks; i += kThreads) {
+            const int in = i % (G / 8), to = i - in + (in % W) * 4 + in / W;
 #pragma unroll 4
-          for (int b = warp; b < cols * blocks; b += kWarps) {
-            const int c = b / blocks, i = (b - c * blocks) * 32 + lane, in = i % (G / 8);
-            const T* row = static_cast<const T*>(a.x) + (jobs.list[first + c] / a.per_row) * a.x_stride + static_cast<int64_t>(s0) * kStep;
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (i < held) v = __ldg(reinterpret_cast<const uint4*>(row) + i);
-            xs[c * a.x_row + i - in + (in % W) * 4 + in / W] =
-                make_uint4(Mma<T>::staged(__byte_perm(v.x, v.z, 0x5410)), Mma<T>::staged(__byte_perm(v.y, v.w, 0x5410)),
-                           Mma<T>::staged(__byte_perm(v.x, v.z, 0x7632)), Mma<T>::staged(__byte_perm(v.y, v.w, 0x7632)));
-            const float2 p = Mma<T>::widen(v.x), q = Mma<T>::widen(v.y), r = Mma<T>::widen(v.z), t = Mma<T>::widen(v.w);
-            float total = ((p.x + p.y) + (q.x + q.y)) + ((r.x + r.y) + (t.x + t.y));
+            for (int c = 0; c < cols; ++c) {
+              uint4 v = make_uint4(0u, 0u, 0u, 0u);
+              if (i < held) v = __ldg(reinterpret_cast<const uint4*>(x_row[c]) + i);
+              xs[c * a.x_row + to] =
+                  make_uint4(Mma<T>::staged(__byte_perm(v.x, v.z, 0x5410)), Mma<T>::staged(__byte_perm(v.y, v.w, 0x5410)),
+                             Mma<T>::staged(__byte_perm(v.x, v.z, 0x7632)), Mma<T>::staged(__byte_perm(v.y, v.w, 0x7632)));
+              const float2 p = Mma<T>::widen(v.x), q = Mma<T>::widen(v.y), r = Mma<T>::widen(v.z), t = Mma<T>::widen(v.w);
+              float total = ((p.x + p.y) + (q.x + q.y)) + ((r.x + r.y) + (t.x + t.y));
 #pragma unroll
-            for (int d = G / 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
-            if (in == 0) xsum[i / (G / 8) * kCols + c] = total;
+              for (int d = G / 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
+              if (in == 0) xsum[i / (G / 8) * kCols + c] = total * (1.0f / Mma<T>::kUnit);
+            }
           }
           __syncthreads();
         }
         open(at);
         const int64_t row = static_cast<int64_t>(jobs.expert[at.job]) * a.N;
-        // low address bits of the scales and zeros of the lane's two rows: where they are in their aligned words
-        int s_low[2], z_low[2];
+        // where the scales of the lane's two rows are in a stage (the same in every step: a step's scales are a multiple of
+        // four bytes), and the low address bits of their zeros
+        int s_at[2], z_low[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t r = static_cast<uint32_t>(row + min(n0 + gid + 8 * h, a.N - 1)) * static_cast<uint32_t>(groups);
-          s_low[h] = static_cast<int>(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.scale)) + r * scale_size);
+          s_at[h] = S::kScales + (gid + 8 * h) * 4 * S::kScaleWords +
+                    static_cast<int>((static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.scale)) + r * scale_size) & 3);
           z_low[h] = ZERO ? static_cast<int>(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.zero)) + r) : 0;
         }
         const uint8_t* x_at[NT];                   // lanes without a column stay on the zeros
@@ -422,8 +437,8 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
           copies_wait<kDepth - 1>();
           __syncwarp();
           const float* const xs_at = xsum + (at.u - s0) * (S::kGroups * kCols) + 2 * quad;
-          if (NT == 1 || cols <= 8) step<T, G, 1, NT, ZERO>(a, stage, x_at, xs_at, at.u, s_low, z_low, gid, quad, sum);
-          else step<T, G, NT, NT, ZERO>(a, stage, x_at, xs_at, at.u, s_low, z_low, gid, quad, sum);
+          if (NT == 1 || cols <= 8) step<T, G, 1, NT, ZERO>(a, stage, x_at, xs_at, at.u, s_at, z_low, gid, quad, sum);
+          else step<T, G, NT, NT, ZERO>(a, stage, x_at, xs_at, at.u, s_at, z_low, gid, quad, sum);
 #pragma unroll
           for (int t = 0; t < NT; ++t) x_at[t] += x_step[t];
           __syncwarp();
@@ -432,6 +447,10 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
         }
       }
 
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[t][k] *= Mma<T>::kUnit;
       if (wk == 1) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -465,10 +484,11 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
 template <typename T, int G, int NT, bool ZERO>
 cudaError_t launch_kernel(MatvecArgs a, cudaStream_t stream) {
   constexpr size_t kRing = static_cast<size_t>(kWarps) * kDepth * Stage<G, ZERO>::kBytes;
-  constexpr size_t kStatic = sizeof(float) * 2 * kWarps * 8 * NT * (kTile + 4) + sizeof(Jobs) + 4 * kWarps;
+  constexpr size_t kStatic = sizeof(float) * 2 * kWarps * 8 * NT * (kTile + 4) + sizeof(Jobs) + 4 * kWarps + 8 * 8 * NT;
   constexpr size_t kX = kSmemMost - kRing - kStatic - 1024 - kStep * 2;      // for staged x and its group sums
   const auto kernel = matvec_w4_kernel<T, G, NT, ZERO>;
-  a.x_cols = a.pairs < 8 * NT ? a.pairs : 8 * NT;
+  const int rows = a.pairs / a.per_row;             // a row that names an expert twice gives it a second job
+  a.x_cols = rows < 8 * NT ? rows : 8 * NT;
   const int steps = (a.K + kStep - 1) / kStep;
   const size_t per_step = static_cast<size_t>(a.x_cols) * kStep * 2 + kStep / G * 8 * NT * 4;
   int slice = static_cast<int>((kX - a.x_cols * 64) / per_step);
