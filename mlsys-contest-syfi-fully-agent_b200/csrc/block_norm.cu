@@ -29,6 +29,7 @@ struct NormArgs {
   const void *x, *y, *gate, *pre_w, *post_w;
   int64_t x_stride, y_stride, gate_stride;   // elements between rows
   int T, H, gate_kind;
+  int arrays, ring;                          // activations that go through the ring, its stages
   int pre_f32, post_f32, gate_f32;           // parameter is fp32 whatever the activations' type is
   float a, eps;
   void *s, *h;                               // [T, H]
@@ -51,31 +52,29 @@ __device__ __forceinline__ int column(int c, int j) {
              : (c * 8 + j) * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x);
 }
 
+// Eight columns of a row as four pairs, zeros behind the row's end.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int c, int H, float (&v)[8]) {
+__device__ __forceinline__ void load8(const T* p, int c, int H, F2 (&v)[4]) {
   if (VEC) {
     const int col = column<VEC>(c, 0);
-    Pack8<T> raw;
     if (col < H) {
-      raw = *reinterpret_cast<const Pack8<T>*>(p + col);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(raw.v[j]);
+      unpack8<T>(*reinterpret_cast<const Pack8<T>*>(p + col), v);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+      for (int j = 0; j < 4; ++j) v[j] = both(0.0f);
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int col = column<VEC>(c, j);
-      v[j] = col < H ? to_f32<T>(p[col]) : 0.0f;
+    for (int j = 0; j < 4; ++j) {
+      const int c0 = column<VEC>(c, 2 * j), c1 = column<VEC>(c, 2 * j + 1);
+      v[j] = make_f2(c0 < H ? to_f32<T>(p[c0]) : 0.0f, c1 < H ? to_f32<T>(p[c1]) : 0.0f);
     }
   }
 }
 
 // A parameter row (weight or gate) in the activations' type or in fp32.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8_param(const void* p, int f32, int64_t row_offset, int c, int H, float (&v)[8]) {
+__device__ __forceinline__ void load8_param(const void* p, int f32, int64_t row_offset, int c, int H, F2 (&v)[4]) {
   if (f32)
     load8<float, VEC>(static_cast<const float*>(p) + row_offset, c, H, v);
   else
@@ -83,111 +82,193 @@ __device__ __forceinline__ void load8_param(const void* p, int f32, int64_t row_
 }
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* p, int c, int H, const float (&v)[8]) {
+__device__ __forceinline__ void store8(T* p, int c, int H, const F2 (&v)[4]) {
   if (VEC) {
     const int col = column<VEC>(c, 0);
-    if (col >= H) return;
-    Pack8<T> raw;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) raw.v[j] = from_f32<T>(v[j]);
-    *reinterpret_cast<Pack8<T>*>(p + col) = raw;
+    if (col < H) *reinterpret_cast<Pack8<T>*>(p + col) = pack8<T>(v);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int col = column<VEC>(c, j);
-      if (col < H) p[col] = from_f32<T>(v[j]);
+    for (int j = 0; j < 4; ++j) {
+      const int c0 = column<VEC>(c, 2 * j), c1 = column<VEC>(c, 2 * j + 1);
+      const float2 f = get(v[j]);
+      if (c0 < H) p[c0] = from_f32<T>(f.x);
+      if (c1 < H) p[c1] = from_f32<T>(f.y);
     }
   }
 }
 
-// One CTA per row; a thread keeps CH groups of eight columns in registers from the loads to the stores.
+template <typename T>
+__device__ __forceinline__ float token_gate(const NormArgs& a, int64_t row) {
+  const int64_t at = row * a.gate_stride;
+  return a.gate_f32 ? static_cast<const float*>(a.gate)[at] : to_f32<T>(static_cast<const T*>(a.gate)[at]);
+}
+
+// ---- Forward
+//
+// Bound by HBM (x, y in; s, h out), so the loads must never wait for the two reductions of a row: persistent CTAs bring
+// the rows of x, y (and a full gate) that they will need through a ring of up to three stages (cp.async).  Every thread copies
+// exactly the sixteen-byte pieces that it will read itself, so the ring needs no barrier.  Weights come from the first-level
+// cache, which the copies pass by.
+constexpr int kMaxRing = 3;
+
+// Until the oldest of `ring` stages in flight has landed.
+__device__ __forceinline__ void ring_wait(int ring) {
+  if (ring == 3) copies_wait<2>();
+  else if (ring == 2) copies_wait<1>();
+  else copies_wait<0>();
+}
+
+// The row's share of one thread in a stage: CH groups of eight columns of up to NARR arrays.
+template <typename T, int CH>
+__device__ __forceinline__ uint32_t piece(int array, int c) {
+  return (array * CH + c) * blockDim.x * sizeof(Pack8<T>) + threadIdx.x * 16;
+}
+
+template <typename T, int CH>
+__device__ __forceinline__ void fetch_row(uint32_t stage, int array, const T* row, int H) {
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int col = column<true>(c, 0);
+    if (col >= H) continue;
+#pragma unroll
+    for (int half = 0; half < static_cast<int>(sizeof(T)) / 2; ++half)
+      copy16(stage + piece<T, CH>(array, c) + half * 16 * blockDim.x, row + col + half * (16 / static_cast<int>(sizeof(T))), true);
+  }
+}
+
+template <typename T, int CH>
+__device__ __forceinline__ void take8(const uint8_t* stage, int array, int c, F2 (&v)[4]) {
+  Pack8<T> raw;
+#pragma unroll
+  for (int half = 0; half < static_cast<int>(sizeof(T)) / 2; ++half)
+    raw.w[half] = *reinterpret_cast<const uint4*>(stage + piece<T, CH>(array, c) + half * 16 * blockDim.x);
+  unpack8<T>(raw, v);
+}
+
+// Pieces behind the row's end are never copied: they hold zeros.
+template <typename T, int CH>
+__device__ __forceinline__ void clear_ring_ends(uint8_t* ring, uint32_t stage_bytes, int stages, int arrays, int H) {
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    if (column<true>(c, 0) < H) continue;
+    for (int i = 0; i < stages * arrays; ++i)
+      for (int half = 0; half < static_cast<int>(sizeof(T)) / 2; ++half)
+        *reinterpret_cast<uint4*>(ring + i / arrays * stage_bytes + piece<T, CH>(i % arrays, c) + half * 16 * blockDim.x) = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+// Where the rows of the kernels without a ring come from: memory.  VEC rows come through the ring.
+template <typename T, int CH, bool VEC>
+__device__ __forceinline__ void row8(const uint8_t* stage, int array, const void* p, int64_t row_offset, int c, int H, F2 (&v)[4]) {
+  if (VEC) take8<T, CH>(stage, array, c, v);
+  else load8<T, false>(static_cast<const T*>(p) + row_offset, c, H, v);
+}
+
 template <typename T, int CH, bool VEC, bool QUANT>
 __global__ void __launch_bounds__(kNormThreads) block_norm_kernel(NormArgs a) {
   griddep_launch_dependents();
   griddep_wait();
+  extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float red[2][32];
   const int H = a.H;
   const float inv_h = 1.0f / static_cast<float>(H);
+  const bool full_in_ring = a.gate_kind == kGateFull && !(a.gate_f32 && sizeof(T) == 2);   // a gate of another type is read directly
+  const uint32_t stage_bytes = static_cast<uint32_t>(a.arrays * CH * blockDim.x * sizeof(Pack8<T>));
+  auto fetch = [&](int64_t row, uint32_t stage) {
+    if (row < a.T) {
+      fetch_row<T, CH>(stage, 0, static_cast<const T*>(a.x) + row * a.x_stride, H);
+      if (a.y) fetch_row<T, CH>(stage, 1, static_cast<const T*>(a.y) + row * a.y_stride, H);
+      if (full_in_ring) fetch_row<T, CH>(stage, 2, static_cast<const T*>(a.gate) + row * a.gate_stride, H);
+    }
+    copies_close();
+  };
+  if (VEC) {
+    clear_ring_ends<T, CH>(ring, stage_bytes, a.ring, a.arrays, H);
+    for (int i = 0; i < a.ring; ++i) fetch(blockIdx.x + static_cast<int64_t>(i) * gridDim.x, smem_address(ring) + i * stage_bytes);
+  }
+  int slot = 0;
   for (int row = blockIdx.x; row < a.T; row += gridDim.x) {
-    float s[CH][8];
+    const uint8_t* const stage = ring + slot * stage_bytes;
+    if (VEC) ring_wait(a.ring);
+    F2 s[CH][4];
     float r1 = 0.0f;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) load8<T, VEC>(static_cast<const T*>(a.x) + row * a.x_stride, c, H, s[c]);
+    for (int c = 0; c < CH; ++c) row8<T, CH, VEC>(stage, 0, a.x, row * a.x_stride, c, H, s[c]);
     if (a.y) {
-      float n[CH][8];
+      F2 n[CH][4];
+      F2 g[4], k = both(1.0f);                     // k: what a whole row of y is multiplied by
 #pragma unroll
-      for (int c = 0; c < CH; ++c) load8<T, VEC>(static_cast<const T*>(a.y) + row * a.y_stride, c, H, n[c]);
+      for (int c = 0; c < CH; ++c) row8<T, CH, VEC>(stage, 1, a.y, row * a.y_stride, c, H, n[c]);
       if (a.post_w) {
-        float sum[1] = {0.0f};
+        F2 square = both(0.0f);
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) sum[0] += n[c][j] * n[c][j];
+          for (int j = 0; j < 4; ++j) square = fma2(n[c][j], n[c][j], square);
+        float sum[1] = {total(square)};
         block_sum(sum, red[0]);
         r1 = rsqrtf(sum[0] * inv_h + a.eps);
+        k = both(r1);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-          float w[8];
-          load8_param<T, VEC>(a.post_w, a.post_f32, 0, c, H, w);
+          load8_param<T, VEC>(a.post_w, a.post_f32, 0, c, H, g);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) n[c][j] = n[c][j] * r1 * w[j];
+          for (int j = 0; j < 4; ++j) n[c][j] = mul2(n[c][j], g[j]);
         }
       }
       if (a.gate_kind == kGateToken) {
-        const int64_t at = row * a.gate_stride;
-        const float g = a.gate_f32 ? static_cast<const float*>(a.gate)[at] : to_f32<T>(static_cast<const T*>(a.gate)[at]);
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) n[c][j] *= g;
+        k = mul2(k, both(token_gate<T>(a, row)));
       } else if (a.gate_kind != kGateNone) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-          float g[8];
-          load8_param<T, VEC>(a.gate, a.gate_f32, a.gate_kind == kGateFull ? row * a.gate_stride : 0, c, H, g);
+          if (VEC && full_in_ring) take8<T, CH>(stage, 2, c, g);
+          else load8_param<T, VEC>(a.gate, a.gate_f32, a.gate_kind == kGateFull ? row * a.gate_stride : 0, c, H, g);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) n[c][j] *= g[j];
+          for (int j = 0; j < 4; ++j) n[c][j] = mul2(n[c][j], g[j]);
         }
       }
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[c][j] = a.a * s[c][j] + n[c][j];
+        for (int j = 0; j < 4; ++j) s[c][j] = fma2(both(a.a), s[c][j], mul2(k, n[c][j]));
         store8<T, VEC>(static_cast<T*>(a.s) + static_cast<int64_t>(row) * H, c, H, s[c]);
       }
     }
-    float sum[1] = {0.0f};
+    if (VEC) {
+      fetch(row + static_cast<int64_t>(a.ring) * gridDim.x, smem_address(stage));
+      slot = slot + 1 == a.ring ? 0 : slot + 1;
+    }
+    F2 square = both(0.0f);
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum[0] += s[c][j] * s[c][j];
+      for (int j = 0; j < 4; ++j) square = fma2(s[c][j], s[c][j], square);
+    float sum[1] = {total(square)};
     block_sum(sum, red[1]);
     const float r2 = rsqrtf(sum[0] * inv_h + a.eps);
-    if (threadIdx.x == 0) {
-      a.rstd[2 * static_cast<int64_t>(row)] = r1;
-      a.rstd[2 * static_cast<int64_t>(row) + 1] = r2;
-    }
+    if (threadIdx.x == 0) *reinterpret_cast<float2*>(a.rstd + 2 * static_cast<int64_t>(row)) = make_float2(r1, r2);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      float w[8];
+      F2 w[4];
       load8_param<T, VEC>(a.pre_w, a.pre_f32, 0, c, H, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[c][j] = s[c][j] * r2 * w[j];
+      for (int j = 0; j < 4; ++j) s[c][j] = mul2(mul2(s[c][j], both(r2)), w[j]);
       if (QUANT) {
         // sixteen lanes hold a block of 128 columns; scale = max(|h|, 1e-10) / 448 and e4m3(h / scale), the rule of the
-        // activation quantiser
+        // activation quantiser, with h times the rounded 1 / scale (at most two roundings of 2^-24 before the one to e4m3)
         const int col = column<true>(c, 0);
         float amax = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(s[c][j]));
+        for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fmaxf(fabsf(get(s[c][j]).x), fabsf(get(s[c][j]).y)));
 #pragma unroll
         for (int d = 8; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
         const float scale = __fdiv_rn(fmaxf(amax, 1e-10f), 448.0f);
-        uint32_t packed[2] = {0u, 0u};
+        const F2 inverse = both(__frcp_rn(scale));
+        uint32_t packed[2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          packed[j >> 2] |= static_cast<uint32_t>(__nv_cvt_float_to_fp8(__fdiv_rn(s[c][j], scale), __NV_SATFINITE, __NV_E4M3))
-                            << (8 * (j & 3));
+        for (int j = 0; j < 2; ++j)
+          packed[j] = __nv_cvt_float2_to_fp8x2(get(mul2(s[c][2 * j], inverse)), __NV_SATFINITE, __NV_E4M3) |
+                      static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(get(mul2(s[c][2 * j + 1], inverse)), __NV_SATFINITE, __NV_E4M3)) << 16;
         if (col < H) {
           *reinterpret_cast<uint2*>(a.q + static_cast<int64_t>(row) * H + col) = make_uint2(packed[0], packed[1]);
           if ((threadIdx.x & 15) == 0) a.q_scale[static_cast<int64_t>(col / kBlock) * a.T + row] = scale;
@@ -202,10 +283,14 @@ __global__ void __launch_bounds__(kNormThreads) block_norm_kernel(NormArgs a) {
   }
 }
 
-// Rows are dealt to the CTAs round-robin; the column sums of a CTA's rows stay in shared memory (every thread owns its
-// columns) and leave once, as one partial row per CTA, which column_sum_kernel adds in CTA order: no atomics, the same
-// bits every time.  The dot products of a row need one reduction: with A = sum u sh, B = sum (gs + r2 u) v and
-// C = sum sh v for v = n (its gate g_t left out of a per-token gate's gradient) everything follows linearly.
+// ---- Backward
+//
+// Rows are dealt to the CTAs round-robin; the column sums of a CTA's rows stay with the thread that owns the columns and
+// leave once, as one partial row per CTA, which column_sum_kernel adds in CTA order: no atomics, the same bits every time.
+// The dot products of a row need one reduction: with D = d - sh k2, d = gs + r2 u and v = n (times a gate per column),
+//     k2 = r2 mean(u sh),   sum_h D v = sum d v - k2 sum sh v,   mean(D g w_post yh) = that (times a gate per token) / H.
+//
+// Two kernels: this one for all cases, with its column sums in shared memory ...
 template <typename T, int CH, bool VEC>
 __global__ void __launch_bounds__(kNormThreads) block_norm_backward_kernel(NormArgs a) {
   griddep_launch_dependents();
@@ -214,72 +299,74 @@ __global__ void __launch_bounds__(kNormThreads) block_norm_backward_kernel(NormA
   __shared__ float red[2][96];
   const int H = a.H, nt = blockDim.x, tid = threadIdx.x;
   const float inv_h = 1.0f / static_cast<float>(H);
+  auto add_to = [&](int sum, int c, int j, F2 v) {
+    float* at = acc + (sum * CH * 8 + c * 8 + 2 * j) * nt + tid;
+    const float2 f = get(v);
+    at[0] += f.x;
+    at[nt] += f.y;
+  };
   for (int i = 0; i < a.n_sums * CH * 8; ++i) acc[i * nt + tid] = 0.0f;
   int flip = 0;
   for (int row = blockIdx.x; row < a.T; row += gridDim.x, flip ^= 1) {
     const float r1 = a.rstd[2 * static_cast<int64_t>(row)], r2 = a.rstd[2 * static_cast<int64_t>(row) + 1];
-    float gt = 1.0f;
-    if (a.gate_kind == kGateToken) {
-      const int64_t at = row * a.gate_stride;
-      gt = a.gate_f32 ? static_cast<const float*>(a.gate)[at] : to_f32<T>(static_cast<const T*>(a.gate)[at]);
-    }
-    float u[CH][8], sh[CH][8], d[CH][8], yh[CH][8];
-    float sums[3] = {0.0f, 0.0f, 0.0f};
+    const float gt = a.gate_kind == kGateToken ? token_gate<T>(a, row) : 1.0f;
+    F2 sh[CH][4], d[CH][4], yh[CH][4];
+    F2 dots[3] = {both(0.0f), both(0.0f), both(0.0f)};
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      float w[8], g[8], wp[8];
+      F2 u[4], w[4], g[4], wp[4];
       load8<T, VEC>(static_cast<const T*>(a.x) + row * a.x_stride, c, H, sh[c]);
-      load8<T, VEC>(static_cast<const T*>(a.gh) + row * a.gh_stride, c, H, u[c]);
+      load8<T, VEC>(static_cast<const T*>(a.gh) + row * a.gh_stride, c, H, u);
       load8_param<T, VEC>(a.pre_w, a.pre_f32, 0, c, H, w);
       if (a.gs) {
         load8<T, VEC>(static_cast<const T*>(a.gs) + row * a.gs_stride, c, H, d[c]);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[c][j] = 0.0f;
+        for (int j = 0; j < 4; ++j) d[c][j] = both(0.0f);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) { g[j] = gt; wp[j] = 1.0f; yh[c][j] = 0.0f; }
+      for (int j = 0; j < 4; ++j) { g[j] = wp[j] = both(1.0f); yh[c][j] = both(0.0f); }
       if (a.y) {
         load8<T, VEC>(static_cast<const T*>(a.y) + row * a.y_stride, c, H, yh[c]);
         if (a.post_w) {
           load8_param<T, VEC>(a.post_w, a.post_f32, 0, c, H, wp);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) yh[c][j] *= r1;
+          for (int j = 0; j < 4; ++j) yh[c][j] = mul2(yh[c][j], both(r1));
         }
         if (a.gate_kind == kGateChannel || a.gate_kind == kGateFull)
           load8_param<T, VEC>(a.gate, a.gate_f32, a.gate_kind == kGateFull ? row * a.gate_stride : 0, c, H, g);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sh[c][j] = a.a * sh[c][j] + g[j] * (yh[c][j] * wp[j]);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        sh[c][j] *= r2;
-        acc[(c * 8 + j) * nt + tid] += u[c][j] * sh[c][j];            // dw_pre
-        u[c][j] *= w[j];
-        d[c][j] += r2 * u[c][j];
-        const float v = yh[c][j] * wp[j] * (a.gate_kind == kGateToken ? 1.0f : g[j]);
-        sums[0] += u[c][j] * sh[c][j];
-        sums[1] += d[c][j] * v;
-        sums[2] += sh[c][j] * v;
+      for (int j = 0; j < 4; ++j) {
+        const F2 v = mul2(mul2(yh[c][j], wp[j]), g[j]);
+        if (a.y) sh[c][j] = fma2(both(a.a), sh[c][j], mul2(both(gt), v));
+        sh[c][j] = mul2(sh[c][j], both(r2));
+        add_to(0, c, j, mul2(u[j], sh[c][j]));            // dw_pre
+        u[j] = mul2(u[j], w[j]);
+        d[c][j] = fma2(both(r2), u[j], d[c][j]);
+        dots[0] = fma2(u[j], sh[c][j], dots[0]);
+        dots[1] = fma2(d[c][j], v, dots[1]);
+        dots[2] = fma2(sh[c][j], v, dots[2]);
       }
     }
+    float sums[3] = {total(dots[0]), total(dots[1]), total(dots[2])};
     block_sum(sums, red[flip]);
-    const float k2 = r2 * (sums[0] * inv_h);                          // D = d - sh k2
-    const float dv = sums[1] - k2 * sums[2];                          // sum_h D v
+    const float k2 = r2 * (sums[0] * inv_h);
+    const float dv = sums[1] - k2 * sums[2];
     if (a.gate_kind == kGateToken && tid == 0) {
       if (a.gate_f32) static_cast<float*>(a.dgate_rows)[row] = dv;
       else static_cast<T*>(a.dgate_rows)[row] = from_f32<T>(dv);
     }
-    const float k1 = dv * gt * inv_h;                                 // mean(D g w_post yh)
+    const float k1 = dv * gt * inv_h;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      float g[8], wp[8], out[8];
+      F2 g[4], wp[4], out[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        d[c][j] -= sh[c][j] * k2;
-        out[j] = a.y ? a.a * d[c][j] : d[c][j];
-        g[j] = gt;
-        wp[j] = 1.0f;
+      for (int j = 0; j < 4; ++j) {
+        d[c][j] = fma2(both(-k2), sh[c][j], d[c][j]);
+        out[j] = a.y ? mul2(both(a.a), d[c][j]) : d[c][j];
+        g[j] = both(gt);
+        wp[j] = both(1.0f);
       }
       store8<T, VEC>(static_cast<T*>(a.dx) + static_cast<int64_t>(row) * H, c, H, out);
       if (!a.y) continue;
@@ -287,21 +374,21 @@ __global__ void __launch_bounds__(kNormThreads) block_norm_backward_kernel(NormA
         load8_param<T, VEC>(a.gate, a.gate_f32, a.gate_kind == kGateFull ? row * a.gate_stride : 0, c, H, g);
       if (a.post_w) load8_param<T, VEC>(a.post_w, a.post_f32, 0, c, H, wp);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) out[j] = d[c][j] * (yh[c][j] * wp[j]);
+      for (int j = 0; j < 4; ++j) out[j] = mul2(d[c][j], mul2(yh[c][j], wp[j]));
       if (a.gate_kind == kGateFull) {
         if (a.gate_f32) store8<float, VEC>(static_cast<float*>(a.dgate_rows) + static_cast<int64_t>(row) * H, c, H, out);
         else store8<T, VEC>(static_cast<T*>(a.dgate_rows) + static_cast<int64_t>(row) * H, c, H, out);
       } else if (a.sum_gate >= 0) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[(a.sum_gate * CH * 8 + c * 8 + j) * nt + tid] += out[j];
+        for (int j = 0; j < 4; ++j) add_to(a.sum_gate, c, j, out[j]);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float dn = d[c][j] * g[j];
+      for (int j = 0; j < 4; ++j) {
+        const F2 dn = mul2(d[c][j], g[j]);
         out[j] = dn;
         if (a.post_w) {
-          acc[(a.sum_post * CH * 8 + c * 8 + j) * nt + tid] += dn * yh[c][j];
-          out[j] = r1 * (dn * wp[j] - yh[c][j] * k1);
+          add_to(a.sum_post, c, j, mul2(dn, yh[c][j]));
+          out[j] = mul2(both(r1), fma2(both(-k1), yh[c][j], mul2(dn, wp[j])));
         }
       }
       store8<T, VEC>(static_cast<T*>(a.dy) + static_cast<int64_t>(row) * H, c, H, out);
@@ -316,6 +403,149 @@ __global__ void __launch_bounds__(kNormThreads) block_norm_backward_kernel(NormA
         const int col = column<VEC>(c, j);
         if (col < H) dst[col] = acc[(k * CH * 8 + c * 8 + j) * nt + tid];
       }
+  }
+}
+
+// ... and this one where rows are aligned, parameters have the activations' type and a row fits 16 columns a thread: the
+// rows come through a ring like the forward's, the column sums stay in registers as fp32, and the weights, which leave no
+// registers for themselves, in shared memory behind the ring (an SM's quarter has 128 registers for each of four warps).
+// Missing parts are neutral values (y = 0, w_post = 1, gate = 1) instead of branches.
+template <typename T, int CH, int MAXT, int GATE>
+__global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) block_norm_backward_ring_kernel(NormArgs a) {
+  griddep_launch_dependents();
+  griddep_wait();
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ float red[2][96];
+  const int H = a.H;
+  const float inv_h = 1.0f / static_cast<float>(H), scale = a.y ? a.a : 1.0f;
+  const uint32_t stage_bytes = static_cast<uint32_t>(a.arrays * CH * blockDim.x * sizeof(Pack8<T>));
+  // arrays of a stage: x, grad_h, grad_stream, y, gate; what the call lacks is never copied and stays zero
+  auto fetch = [&](int64_t row, uint32_t stage) {
+    if (row < a.T) {
+      fetch_row<T, CH>(stage, 0, static_cast<const T*>(a.x) + row * a.x_stride, H);
+      fetch_row<T, CH>(stage, 1, static_cast<const T*>(a.gh) + row * a.gh_stride, H);
+      if (a.gs) fetch_row<T, CH>(stage, 2, static_cast<const T*>(a.gs) + row * a.gs_stride, H);
+      if (a.y) fetch_row<T, CH>(stage, 3, static_cast<const T*>(a.y) + row * a.y_stride, H);
+      if (GATE == kGateFull) fetch_row<T, CH>(stage, 4, static_cast<const T*>(a.gate) + row * a.gate_stride, H);
+    }
+    copies_close();
+  };
+  for (uint32_t i = threadIdx.x * 16; i < a.ring * stage_bytes; i += blockDim.x * 16) *reinterpret_cast<uint4*>(ring + i) = make_uint4(0u, 0u, 0u, 0u);
+  __syncthreads();
+  for (int i = 0; i < a.ring; ++i) fetch(blockIdx.x + static_cast<int64_t>(i) * gridDim.x, smem_address(ring) + i * stage_bytes);
+
+  uint8_t* const weights = ring + a.ring * stage_bytes;    // w_pre, w_post, gate per channel: the thread's own pieces
+  F2 sum_pre[CH][4], sum_post[CH][4], sum_gate[GATE == kGateChannel ? CH : 1][4];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int col = column<true>(c, 0);
+    const F2 ones[4] = {both(1.0f), both(1.0f), both(1.0f), both(1.0f)};
+    const void* const from[3] = {a.pre_w, a.post_w, GATE == kGateChannel ? a.gate : nullptr};
+#pragma unroll
+    for (int k = 0; k < (GATE == kGateChannel ? 3 : 2); ++k) {
+      const Pack8<T> v = from[k] && col < H ? *reinterpret_cast<const Pack8<T>*>(static_cast<const T*>(from[k]) + col) : pack8<T>(ones);
+#pragma unroll
+      for (int half = 0; half < static_cast<int>(sizeof(T)) / 2; ++half)
+        *reinterpret_cast<uint4*>(weights + piece<T, CH>(k, c) + half * 16 * blockDim.x) = v.w[half];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      sum_pre[c][j] = sum_post[c][j] = both(0.0f);
+      if (GATE == kGateChannel) sum_gate[c][j] = both(0.0f);
+    }
+  }
+
+  // a row's statistics and gate are loaded a row ahead
+  auto stats = [&](int64_t row, float& r1, float& r2, float& gt) {
+    r1 = r2 = gt = 1.0f;
+    if (row >= a.T) return;
+    const float2 r = *reinterpret_cast<const float2*>(a.rstd + 2 * row);
+    r2 = r.y;
+    if (a.post_w) r1 = r.x;
+    if (GATE == kGateNone && a.gate_kind == kGateToken) gt = token_gate<T>(a, row);
+  };
+  float next_r1, next_r2, next_gt;
+  stats(blockIdx.x, next_r1, next_r2, next_gt);
+  int flip = 0, slot = 0;
+  for (int row = blockIdx.x; row < a.T; row += gridDim.x, flip ^= 1) {
+    const uint8_t* const stage = ring + slot * stage_bytes;
+    const float r1 = next_r1, r2 = next_r2, gt = next_gt;
+    stats(row + static_cast<int64_t>(gridDim.x), next_r1, next_r2, next_gt);
+    ring_wait(a.ring);
+    F2 sh[CH][4], d[CH][4];
+    F2 dots[3] = {both(0.0f), both(0.0f), both(0.0f)};
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      F2 u[4], w[4], g[4], wp[4], yh[4];
+      take8<T, CH>(stage, 0, c, sh[c]);
+      take8<T, CH>(stage, 1, c, u);
+      take8<T, CH>(stage, 2, c, d[c]);
+      take8<T, CH>(stage, 3, c, yh);
+      take8<T, CH>(weights, 0, c, w);
+      take8<T, CH>(weights, 1, c, wp);
+      if (GATE == kGateChannel) take8<T, CH>(weights, 2, c, g);
+      if (GATE == kGateFull) take8<T, CH>(stage, 4, c, g);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        F2 v = mul2(mul2(yh[j], both(r1)), wp[j]);
+        if (GATE != kGateNone) v = mul2(v, g[j]);
+        sh[c][j] = mul2(fma2(both(scale), sh[c][j], GATE == kGateNone ? mul2(both(gt), v) : v), both(r2));
+        sum_pre[c][j] = fma2(u[j], sh[c][j], sum_pre[c][j]);
+        u[j] = mul2(u[j], w[j]);
+        d[c][j] = fma2(both(r2), u[j], d[c][j]);
+        dots[0] = fma2(u[j], sh[c][j], dots[0]);
+        dots[1] = fma2(d[c][j], v, dots[1]);
+        dots[2] = fma2(sh[c][j], v, dots[2]);
+      }
+    }
+    float sums[3] = {total(dots[0]), total(dots[1]), total(dots[2])};
+    block_sum(sums, red[flip]);
+    const float k2 = r2 * (sums[0] * inv_h);
+    const float dv = sums[1] - k2 * sums[2];
+    if (GATE == kGateNone && a.gate_kind == kGateToken && threadIdx.x == 0) static_cast<T*>(a.dgate_rows)[row] = from_f32<T>(dv);
+    const float k1 = a.post_w ? dv * gt * inv_h * r1 : 0.0f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      F2 g[4], wp[4], out[4], yh[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        d[c][j] = fma2(both(-k2), sh[c][j], d[c][j]);
+        out[j] = mul2(both(scale), d[c][j]);
+      }
+      store8<T, true>(static_cast<T*>(a.dx) + static_cast<int64_t>(row) * H, c, H, out);
+      if (!a.y) continue;
+      take8<T, CH>(stage, 3, c, yh);               // read again: registers are what this kernel is short of
+      take8<T, CH>(weights, 1, c, wp);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) yh[j] = mul2(yh[j], both(r1));
+      if (GATE == kGateChannel) take8<T, CH>(weights, 2, c, g);
+      if (GATE == kGateFull) take8<T, CH>(stage, 4, c, g);
+      if (GATE != kGateNone) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const F2 n = mul2(yh[j], wp[j]);
+          if (GATE == kGateChannel) sum_gate[c][j] = fma2(d[c][j], n, sum_gate[c][j]);
+          else out[j] = mul2(d[c][j], n);
+        }
+        if (GATE == kGateFull) store8<T, true>(static_cast<T*>(a.dgate_rows) + static_cast<int64_t>(row) * H, c, H, out);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const F2 dn = mul2(d[c][j], GATE == kGateNone ? both(gt) : g[j]);
+        sum_post[c][j] = fma2(dn, yh[j], sum_post[c][j]);
+        out[j] = fma2(both(-k1), yh[j], mul2(mul2(dn, wp[j]), both(r1)));
+      }
+      store8<T, true>(static_cast<T*>(a.dy) + static_cast<int64_t>(row) * H, c, H, out);
+    }
+    fetch(row + static_cast<int64_t>(a.ring) * gridDim.x, smem_address(stage));
+    slot = slot + 1 == a.ring ? 0 : slot + 1;
+  }
+  float* dst = a.partial + static_cast<int64_t>(blockIdx.x) * a.n_sums * H;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    store8<float, true>(dst, c, H, sum_pre[c]);
+    if (a.sum_post >= 0) store8<float, true>(dst + static_cast<int64_t>(a.sum_post) * H, c, H, sum_post[c]);
+    if (GATE == kGateChannel) store8<float, true>(dst + static_cast<int64_t>(a.sum_gate) * H, c, H, sum_gate[c]);
   }
 }
 
@@ -338,7 +568,7 @@ __global__ void __launch_bounds__(32 * kSumStrips) column_sum_kernel(ColumnSumAr
   const int col = blockIdx.x * 32 + lane;
   float s = 0.0f;
   if (col < a.H) {
-#pragma unroll 4
+#pragma unroll 8
     for (int p = w; p < a.n_parts; p += kSumStrips) s += a.partial[(static_cast<int64_t>(p) * a.n_sums + k) * a.H + col];
   }
   strip[w][lane] = s;
@@ -383,14 +613,41 @@ bool bad_common(const NormArgs& a, int dtype, int param_f32) {
          (a.post_w && !a.y);
 }
 
+constexpr size_t kRingMost = 208 * 1024;          // shared memory of an SM for rings; the rest is first-level cache
+
 int grid_rows(int T, int per_sm) { return T < kNumSMs * per_sm ? T : kNumSMs * per_sm; }
+
+// Activations that a row's ring stage holds: x, y and a full gate of the same type.
+int forward_arrays(const NormArgs& a, int size) {
+  return 1 + (a.y ? 1 : 0) + (a.gate_kind == kGateFull && (!a.gate_f32 || size == 4) ? 1 : 0);
+}
+
+template <typename T, int CH, bool VEC, bool QUANT>
+cudaError_t launch_forward(NormArgs a, int threads, cudaStream_t stream) {
+  const auto kernel = block_norm_kernel<T, CH, VEC, QUANT>;
+  size_t smem = 0;
+  int per_sm = 8;
+  if (VEC) {
+    a.arrays = forward_arrays(a, sizeof(T));
+    const size_t stage = static_cast<size_t>(a.arrays) * CH * threads * sizeof(Pack8<T>);
+    // as many CTAs as the registers hold (72 a thread), or fewer where their rings do not fit; two stages at least, if
+    // that can be had
+    per_sm = 896 / threads > 0 ? 896 / threads : 1;
+    while (per_sm > 1 && 2 * stage * per_sm > kRingMost) per_sm /= 2;
+    a.ring = static_cast<int>(kRingMost / (stage * per_sm));
+    if (a.ring > kMaxRing) a.ring = kMaxRing;
+    smem = a.ring * stage;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+  }
+  return launch_pdl(kernel, dim3(grid_rows(a.T, per_sm)), dim3(threads), smem, stream, a);
+}
 
 template <typename T, int CH>
 cudaError_t launch_forward(const NormArgs& a, bool vec, int threads, cudaStream_t stream) {
-  const dim3 grid(grid_rows(a.T, 8)), block(threads);
-  if (a.q) return launch_pdl(block_norm_kernel<T, CH, true, true>, grid, block, 0, stream, a);
-  if (vec) return launch_pdl(block_norm_kernel<T, CH, true, false>, grid, block, 0, stream, a);
-  return launch_pdl(block_norm_kernel<T, CH, false, false>, grid, block, 0, stream, a);
+  if (a.q) return launch_forward<T, CH, true, true>(a, threads, stream);
+  if (vec) return launch_forward<T, CH, true, false>(a, threads, stream);
+  return launch_forward<T, CH, false, false>(a, threads, stream);
 }
 
 template <typename T>
@@ -401,28 +658,63 @@ cudaError_t launch_forward(const NormArgs& a, bool vec, cudaStream_t stream) {
   return launch_forward<T, 4>(a, vec, sh.threads, stream);
 }
 
+// CTAs of the backward pass, one partial row of column sums each: as many as the registers hold.
+int backward_parts(int T, int H) {
+  const Shape sh = shape_of(H);
+  return grid_rows(T, sh.ch > 1 ? 1 : 512 / sh.threads);
+}
+
 template <typename T, int CH, bool VEC>
 cudaError_t launch_backward(const NormArgs& a, int grid, int threads, cudaStream_t stream) {
   const size_t smem = static_cast<size_t>(a.n_sums) * CH * 8 * threads * sizeof(float);
-  cudaError_t e = cudaFuncSetAttribute(block_norm_backward_kernel<T, CH, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(smem));
+  const cudaError_t e = cudaFuncSetAttribute(block_norm_backward_kernel<T, CH, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(smem));
   if (e != cudaSuccess) return e;
   return launch_pdl(block_norm_backward_kernel<T, CH, VEC>, dim3(grid), dim3(threads), smem, stream, a);
 }
 
+template <typename T, int CH, int MAXT, int GATE>
+cudaError_t launch_ring(const NormArgs& a, int grid, int threads, size_t smem, cudaStream_t stream) {
+  const auto kernel = block_norm_backward_ring_kernel<T, CH, MAXT, GATE>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kernel, dim3(grid), dim3(threads), smem, stream, a);
+}
+
+template <typename T, int CH, int MAXT>
+cudaError_t launch_ring(const NormArgs& a, int grid, int threads, size_t smem, cudaStream_t stream) {
+  if (a.gate_kind == kGateChannel) return launch_ring<T, CH, MAXT, kGateChannel>(a, grid, threads, smem, stream);
+  if (a.gate_kind == kGateFull) return launch_ring<T, CH, MAXT, kGateFull>(a, grid, threads, smem, stream);
+  return launch_ring<T, CH, MAXT, kGateNone>(a, grid, threads, smem, stream);
+}
+
 template <typename T>
-cudaError_t launch_backward(const NormArgs& a, const ColumnSumArgs& cs, bool vec, cudaStream_t stream) {
+cudaError_t launch_backward(NormArgs a, const ColumnSumArgs& cs, bool vec, cudaStream_t stream) {
   const Shape sh = shape_of(a.H);
   const int grid = cs.n_parts, nt = sh.threads;
+  a.arrays = a.gate_kind == kGateFull ? 5 : 4;
+  const size_t array = static_cast<size_t>(sh.ch) * nt * sizeof(Pack8<T>), stage = a.arrays * array, weights = 3 * array;
+  const bool own_type = sizeof(T) == 4 || !(a.pre_f32 || a.post_f32 || a.gate_f32);
+  // the ring kernel wants two stages at least; a longer row or a mixed call takes the other one
+  const size_t room = 220 * 1024 / (sh.ch == 1 ? 512 / nt : 1) - 2048;
+  a.ring = room > weights ? static_cast<int>((room - weights) / stage) : 0;
+  if (a.ring > kMaxRing) a.ring = kMaxRing;
   cudaError_t e;
-  if (sh.ch == 1) e = vec ? launch_backward<T, 1, true>(a, grid, nt, stream) : launch_backward<T, 1, false>(a, grid, nt, stream);
-  else if (sh.ch == 2) e = vec ? launch_backward<T, 2, true>(a, grid, nt, stream) : launch_backward<T, 2, false>(a, grid, nt, stream);
-  else e = vec ? launch_backward<T, 4, true>(a, grid, nt, stream) : launch_backward<T, 4, false>(a, grid, nt, stream);
+  if (vec && own_type && sh.ch <= 2 && a.ring >= 2) {
+    const size_t smem = a.ring * stage + weights;
+    if (sh.ch == 1) e = launch_ring<T, 1, 256>(a, grid, nt, smem, stream);
+    else e = launch_ring<T, 2, 512>(a, grid, nt, smem, stream);
+  } else if (sh.ch == 1) {
+    e = vec ? launch_backward<T, 1, true>(a, grid, nt, stream) : launch_backward<T, 1, false>(a, grid, nt, stream);
+  } else if (sh.ch == 2) {
+    e = vec ? launch_backward<T, 2, true>(a, grid, nt, stream) : launch_backward<T, 2, false>(a, grid, nt, stream);
+  } else {
+    e = vec ? launch_backward<T, 4, true>(a, grid, nt, stream) : launch_backward<T, 4, false>(a, grid, nt, stream);
+  }
   if (e != cudaSuccess) return e;
   return launch_pdl(column_sum_kernel<T>, dim3((a.H + 31) / 32, cs.n_sums), dim3(32 * kSumStrips), 0, stream, cs);
 }
 
-int backward_parts(int T) { return grid_rows(T, 1); }
 
 }  // namespace
 }  // namespace moe
@@ -461,7 +753,7 @@ extern "C" int moe_fp8_block_scale_block_norm(const void* x, int64_t x_stride, c
 
 extern "C" size_t moe_fp8_block_scale_block_norm_backward_workspace_bytes(int T, int H) {
   if (T < 0 || H < 1 || H > kMaxWidth) return 0;
-  return static_cast<size_t>(backward_parts(T)) * 3 * H * sizeof(float);
+  return static_cast<size_t>(backward_parts(T, H)) * 3 * H * sizeof(float);
 }
 
 extern "C" int moe_fp8_block_scale_block_norm_backward(
@@ -503,7 +795,7 @@ extern "C" int moe_fp8_block_scale_block_norm_backward(
   }
   a.partial = static_cast<float*>(workspace);
   cs.partial = a.partial;
-  cs.n_parts = backward_parts(T);
+  cs.n_parts = backward_parts(T, H);
   cs.n_sums = a.n_sums;
   cs.H = H;
   const bool vec = vector_rows(a, dtype);

@@ -82,16 +82,6 @@ template <> struct Words<4> { using Type = uint4; };
 template <> struct Words<2> { using Type = uint2; };
 template <> struct Words<1> { using Type = uint32_t; };
 
-__device__ __forceinline__ uint32_t smem_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy4(uint32_t to, const void* from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copies_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // A stage: 16 rows of 128 bytes of weights (16-byte chunks swizzled by row, so that 4-, 8- and 16-byte reads of eight rows
 // are free of bank conflicts), then per row the aligned words that hold its scales, then those with its zero points.
 template <int G, bool ZERO> struct Stage {
