@@ -164,31 +164,57 @@ __device__ __forceinline__ void row8(const uint8_t* stage, int array, const void
   else load8<T, false>(static_cast<const T*>(p) + row_offset, c, H, v);
 }
 
-template <typename T, int CH, bool VEC, bool QUANT>
-__global__ void __launch_bounds__(kNormThreads) block_norm_kernel(NormArgs a) {
+// GATE: where the gate and the parameters' types are known (all of the activations' type), else kAnyGate.
+constexpr int kAnyGate = -1;
+
+template <typename T, int CH, bool VEC, bool QUANT, int GATE>
+__global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, !VEC ? 1 : CH == 1 ? 3 : CH == 2 ? 2 : 1) block_norm_kernel(NormArgs a) {
   griddep_launch_dependents();
   griddep_wait();
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float red[2][32];
   const int H = a.H;
+  const int gate_kind = GATE == kAnyGate ? a.gate_kind : GATE == kGateNone && a.gate_kind == kGateToken ? kGateToken : GATE;
   const float inv_h = 1.0f / static_cast<float>(H);
-  const bool full_in_ring = a.gate_kind == kGateFull && !(a.gate_f32 && sizeof(T) == 2);   // a gate of another type is read directly
+  // a full gate of another type than the activations' is read directly
+  const bool full_in_ring = GATE == kGateFull || (GATE == kAnyGate && gate_kind == kGateFull && !(a.gate_f32 && sizeof(T) == 2));
   const uint32_t stage_bytes = static_cast<uint32_t>(a.arrays * CH * blockDim.x * sizeof(Pack8<T>));
-  auto fetch = [&](int64_t row, uint32_t stage) {
-    if (row < a.T) {
-      fetch_row<T, CH>(stage, 0, static_cast<const T*>(a.x) + row * a.x_stride, H);
-      if (a.y) fetch_row<T, CH>(stage, 1, static_cast<const T*>(a.y) + row * a.y_stride, H);
-      if (full_in_ring) fetch_row<T, CH>(stage, 2, static_cast<const T*>(a.gate) + row * a.gate_stride, H);
+  auto param = [&](const void* p, int f32, int64_t offset, int c, F2 (&v)[4]) {
+    if (GATE == kAnyGate) load8_param<T, VEC>(p, f32, offset, c, H, v);
+    else load8<T, VEC>(static_cast<const T*>(p) + offset, c, H, v);
+  };
+  // rows still to be fetched and to be stored
+  int64_t fetch_at = blockIdx.x;
+  const T* fetch_x = static_cast<const T*>(a.x) + fetch_at * a.x_stride;
+  const T* fetch_y = static_cast<const T*>(a.y) + fetch_at * a.y_stride;
+  const T* fetch_g = static_cast<const T*>(a.gate) + fetch_at * a.gate_stride;
+  const int64_t step = gridDim.x;
+  auto fetch = [&](uint32_t stage) {
+    if (fetch_at < a.T) {
+      fetch_row<T, CH>(stage, 0, fetch_x, H);
+      if (a.y) fetch_row<T, CH>(stage, 1, fetch_y, H);
+      if (full_in_ring) fetch_row<T, CH>(stage, 2, fetch_g, H);
     }
+    fetch_at += step;
+    fetch_x += step * a.x_stride;
+    fetch_y += step * a.y_stride;
+    fetch_g += step * a.gate_stride;
     copies_close();
   };
   if (VEC) {
     clear_ring_ends<T, CH>(ring, stage_bytes, a.ring, a.arrays, H);
-    for (int i = 0; i < a.ring; ++i) fetch(blockIdx.x + static_cast<int64_t>(i) * gridDim.x, smem_address(ring) + i * stage_bytes);
+    for (int i = 0; i < a.ring; ++i) fetch(smem_address(ring) + i * stage_bytes);
   }
+  T* s_out = static_cast<T*>(a.s) + blockIdx.x * static_cast<int64_t>(H);
+  T* h_out = static_cast<T*>(a.h) + blockIdx.x * static_cast<int64_t>(H);
+  uint8_t* q_out = a.q + blockIdx.x * static_cast<int64_t>(H);
+  const int64_t step_h = step * H;
+  float next_gate = gate_kind == kGateToken && blockIdx.x < a.T ? token_gate<T>(a, blockIdx.x) : 1.0f;   // loaded a row ahead
   int slot = 0;
   for (int row = blockIdx.x; row < a.T; row += gridDim.x) {
     const uint8_t* const stage = ring + slot * stage_bytes;
+    const float gate = next_gate;
+    if (gate_kind == kGateToken && row + step < a.T) next_gate = token_gate<T>(a, row + step);
     if (VEC) ring_wait(a.ring);
     F2 s[CH][4];
     float r1 = 0.0f;
@@ -196,7 +222,8 @@ __global__ void __launch_bounds__(kNormThreads) block_norm_kernel(NormArgs a) {
     for (int c = 0; c < CH; ++c) row8<T, CH, VEC>(stage, 0, a.x, row * a.x_stride, c, H, s[c]);
     if (a.y) {
       F2 n[CH][4];
-      F2 g[4], k = both(1.0f);                     // k: what a whole row of y is multiplied by
+      F2 g[4];
+      float k = gate;                              // what a whole row of y is multiplied by
 #pragma unroll
       for (int c = 0; c < CH; ++c) row8<T, CH, VEC>(stage, 1, a.y, row * a.y_stride, c, H, n[c]);
       if (a.post_w) {
@@ -208,34 +235,33 @@ __global__ void __launch_bounds__(kNormThreads) block_norm_kernel(NormArgs a) {
         float sum[1] = {total(square)};
         block_sum(sum, red[0]);
         r1 = rsqrtf(sum[0] * inv_h + a.eps);
-        k = both(r1);
+        k *= r1;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-          load8_param<T, VEC>(a.post_w, a.post_f32, 0, c, H, g);
+          param(a.post_w, a.post_f32, 0, c, g);
 #pragma unroll
           for (int j = 0; j < 4; ++j) n[c][j] = mul2(n[c][j], g[j]);
         }
       }
-      if (a.gate_kind == kGateToken) {
-        k = mul2(k, both(token_gate<T>(a, row)));
-      } else if (a.gate_kind != kGateNone) {
+      if (gate_kind == kGateChannel || gate_kind == kGateFull) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
           if (VEC && full_in_ring) take8<T, CH>(stage, 2, c, g);
-          else load8_param<T, VEC>(a.gate, a.gate_f32, a.gate_kind == kGateFull ? row * a.gate_stride : 0, c, H, g);
+          else param(a.gate, a.gate_f32, gate_kind == kGateFull ? row * a.gate_stride : 0, c, g);
 #pragma unroll
           for (int j = 0; j < 4; ++j) n[c][j] = mul2(n[c][j], g[j]);
         }
       }
+      const F2 kk = both(k), aa = both(a.a);
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[c][j] = fma2(both(a.a), s[c][j], mul2(k, n[c][j]));
-        store8<T, VEC>(static_cast<T*>(a.s) + static_cast<int64_t>(row) * H, c, H, s[c]);
+        for (int j = 0; j < 4; ++j) s[c][j] = fma2(aa, s[c][j], mul2(kk, n[c][j]));
+        store8<T, VEC>(s_out, c, H, s[c]);
       }
     }
     if (VEC) {
-      fetch(row + static_cast<int64_t>(a.ring) * gridDim.x, smem_address(stage));
+      fetch(smem_address(stage));
       slot = slot + 1 == a.ring ? 0 : slot + 1;
     }
     F2 square = both(0.0f);
@@ -247,36 +273,39 @@ __global__ void __launch_bounds__(kNormThreads) block_norm_kernel(NormArgs a) {
     block_sum(sum, red[1]);
     const float r2 = rsqrtf(sum[0] * inv_h + a.eps);
     if (threadIdx.x == 0) *reinterpret_cast<float2*>(a.rstd + 2 * static_cast<int64_t>(row)) = make_float2(r1, r2);
+    const F2 rr = both(r2);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       F2 w[4];
-      load8_param<T, VEC>(a.pre_w, a.pre_f32, 0, c, H, w);
+      param(a.pre_w, a.pre_f32, 0, c, w);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[c][j] = mul2(mul2(s[c][j], both(r2)), w[j]);
+      for (int j = 0; j < 4; ++j) s[c][j] = mul2(mul2(s[c][j], rr), w[j]);
       if (QUANT) {
         // sixteen lanes hold a block of 128 columns; scale = max(|h|, 1e-10) / 448 and e4m3(h / scale), the rule of the
-        // activation quantiser, with h times the rounded 1 / scale (at most two roundings of 2^-24 before the one to e4m3)
+        // activation quantiser, with products of reciprocals (errors of 2^-22 before the rounding to e4m3's 2^-4)
         const int col = column<true>(c, 0);
-        float amax = 0.0f;
+        float amax = 1e-10f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fmaxf(fabsf(get(s[c][j]).x), fabsf(get(s[c][j]).y)));
 #pragma unroll
         for (int d = 8; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
-        const float scale = __fdiv_rn(fmaxf(amax, 1e-10f), 448.0f);
-        const F2 inverse = both(__frcp_rn(scale));
+        const F2 inverse = both(__fdividef(448.0f, amax));
         uint32_t packed[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
           packed[j] = __nv_cvt_float2_to_fp8x2(get(mul2(s[c][2 * j], inverse)), __NV_SATFINITE, __NV_E4M3) |
                       static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(get(mul2(s[c][2 * j + 1], inverse)), __NV_SATFINITE, __NV_E4M3)) << 16;
         if (col < H) {
-          *reinterpret_cast<uint2*>(a.q + static_cast<int64_t>(row) * H + col) = make_uint2(packed[0], packed[1]);
-          if ((threadIdx.x & 15) == 0) a.q_scale[static_cast<int64_t>(col / kBlock) * a.T + row] = scale;
+          *reinterpret_cast<uint2*>(q_out + col) = make_uint2(packed[0], packed[1]);
+          if ((threadIdx.x & 15) == 0) a.q_scale[static_cast<int64_t>(col / kBlock) * a.T + row] = amax * (1.0f / 448.0f);
         }
       } else {
-        store8<T, VEC>(static_cast<T*>(a.h) + static_cast<int64_t>(row) * H, c, H, s[c]);
+        store8<T, VEC>(h_out, c, H, s[c]);
       }
     }
+    s_out += step_h;
+    h_out += step_h;
+    q_out += step_h;
     // red[0] of the next row is written only after every thread has passed the barrier of red[1], and without a first
     // sum red[1] would be written again while a slow thread reads it
     if (!a.post_w) __syncthreads();
@@ -622,15 +651,15 @@ int forward_arrays(const NormArgs& a, int size) {
   return 1 + (a.y ? 1 : 0) + (a.gate_kind == kGateFull && (!a.gate_f32 || size == 4) ? 1 : 0);
 }
 
-template <typename T, int CH, bool VEC, bool QUANT>
+template <typename T, int CH, bool VEC, bool QUANT, int GATE>
 cudaError_t launch_forward(NormArgs a, int threads, cudaStream_t stream) {
-  const auto kernel = block_norm_kernel<T, CH, VEC, QUANT>;
+  const auto kernel = block_norm_kernel<T, CH, VEC, QUANT, GATE>;
   size_t smem = 0;
   int per_sm = 8;
   if (VEC) {
     a.arrays = forward_arrays(a, sizeof(T));
     const size_t stage = static_cast<size_t>(a.arrays) * CH * threads * sizeof(Pack8<T>);
-    // as many CTAs as the registers hold (72 a thread), or fewer where their rings do not fit; two stages at least, if
+    // as many CTAs as the registers are cut for, or fewer where their rings do not fit; two stages at least, if
     // that can be had
     per_sm = 896 / threads > 0 ? 896 / threads : 1;
     while (per_sm > 1 && 2 * stage * per_sm > kRingMost) per_sm /= 2;
@@ -643,11 +672,23 @@ cudaError_t launch_forward(NormArgs a, int threads, cudaStream_t stream) {
   return launch_pdl(kernel, dim3(grid_rows(a.T, per_sm)), dim3(threads), smem, stream, a);
 }
 
+template <typename T, int CH, bool QUANT>
+cudaError_t launch_forward(const NormArgs& a, int threads, cudaStream_t stream) {
+  const bool own_type = sizeof(T) == 4 || !(a.pre_f32 || a.post_f32 || a.gate_f32);
+  if (own_type && CH <= 2) {
+    constexpr int kCh = CH <= 2 ? CH : 1;
+    if (a.gate_kind == kGateChannel) return launch_forward<T, kCh, true, QUANT, kGateChannel>(a, threads, stream);
+    if (a.gate_kind == kGateFull) return launch_forward<T, kCh, true, QUANT, kGateFull>(a, threads, stream);
+    return launch_forward<T, kCh, true, QUANT, kGateNone>(a, threads, stream);
+  }
+  return launch_forward<T, CH, true, QUANT, kAnyGate>(a, threads, stream);
+}
+
 template <typename T, int CH>
 cudaError_t launch_forward(const NormArgs& a, bool vec, int threads, cudaStream_t stream) {
-  if (a.q) return launch_forward<T, CH, true, true>(a, threads, stream);
-  if (vec) return launch_forward<T, CH, true, false>(a, threads, stream);
-  return launch_forward<T, CH, false, false>(a, threads, stream);
+  if (a.q) return launch_forward<T, CH, true>(a, threads, stream);
+  if (vec) return launch_forward<T, CH, false>(a, threads, stream);
+  return launch_forward<T, CH, false, false, kAnyGate>(a, threads, stream);
 }
 
 template <typename T>
