@@ -268,7 +268,7 @@ int moe_fp8_block_scale_route_static(const float* routing_logits, const uint16_t
  *   x, y [T, H] (y may be NULL), H <= 16384; pre_weight [H]; post_weight [H] or NULL (needs y)
  *   gate_kind 0: none, 1: [H] per channel, 2: [T] per token (gate_stride apart), 3: [T, H]; needs y
  *   param_f32: bit 0 / 1 / 2 set: pre_weight / post_weight / gate are fp32, else they have x's type
- *   stream_out [T, H] = s (only with y); rstd f32 [T, 2] = (r1 or 0, r2), which the backward takes
+ *   stream_out [T, H] = s (only with y); rstd f32 [T, 2] (8-byte aligned) = (r1 or 0, r2), which the backward takes
  *   h_scale NULL: h [T, H] in x's type.  h_scale given: the shard's input, h e4m3 [T, H] and h_scale f32 [H / 128, T]
  *   (max(|h|, 1e-10) / 448 per 128 columns, from the unrounded h); H a multiple of 128, rows 16-byte aligned.
  * Everything in between is fp32; what is stored is rounded once, h comes from the unrounded s. */

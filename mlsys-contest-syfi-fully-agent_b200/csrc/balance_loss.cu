@@ -7,19 +7,23 @@
 //     dloss/dz_ti = alpha E / (K n^2) d_ti (c_i - sum_j c_j p_tj),    d = p (1 - s) for sigmoid, p for softmax.
 // A row whose scores are all zero (every logit -inf) has p = 0 and no gradient.
 //
-// One warp takes a token: lane l holds experts l, l + 32, ...  The token axis is cut into equal chunks, one CTA each; a
-// CTA walks through the sequences that meet its chunk.  What lies inside the chunk is finished there; a sequence that
-// crosses a border leaves one partial row per chunk, which balance_join_kernel adds in chunk order (no floating-point
-// atomics: the same bits every time).  Counts are integers.
+// Forward: the token axis is cut into equal chunks, one CTA of up to 32 warps each, a warp per token.  A sequence of up to 8
+// tokens inside the chunk is one warp's work from its probabilities to its loss; a longer one is the whole CTA's.  What
+// lies inside the chunk is finished there; a sequence that crosses a border leaves one partial row per chunk, which
+// balance_join_kernel adds in chunk order (no floating-point atomics: the same bits every time).  Counts are integers.
+// Bound by latency (search of the borders, load, reductions) up to some thousand tokens and by the exponentials and
+// their reductions beyond; a row is loaded while the one before is worked on.
 #include "elem_device.cuh"
 
 namespace moe {
 namespace {
 
 constexpr int kMaxExperts = 1024;
-constexpr int kChunkWarps = 8;
+// Warps of a chunk's CTA: what the registers of its lanes' experts leave.
+__host__ __device__ constexpr int chunk_warps(int per_lane) { return per_lane <= 8 ? 32 : per_lane <= 16 ? 16 : 8; }
 constexpr int kMinChunk = 32;          // tokens; smaller batches stay in one CTA, which needs no second launch
-constexpr int kMaxChunks = 4 * kNumSMs;
+constexpr int kShort = 8;              // longest sequence that one warp takes
+constexpr int kBackWarps = 8;
 
 struct BalanceArgs {
   const void* logits;
@@ -61,90 +65,189 @@ __device__ __forceinline__ int begun_before(const BalanceArgs& a, int t, int lan
   return lo;
 }
 
-// Probabilities of a row, zero where the row has none, and in s what the slope dp/dz needs beside them: 1 - sigmoid(z)
-// (1 for a softmax), formed as e^-z sigmoid(z) where 1 - sigmoid(z) would cancel.
-template <typename T, int EPL>
-__device__ __forceinline__ void probabilities(const BalanceArgs& a, int t, int lane, float (&s)[EPL], float (&p)[EPL]) {
+// Expert of a lane's i-th value: neighbours where a row can be read 16 bytes at a time, else 32 apart.
+template <typename T, bool VEC>
+__device__ __forceinline__ int expert_of(int i, int lane) {
+  constexpr int kRun = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+  return (i / kRun * 32 + lane) * kRun + i % kRun;
+}
+
+// A lane's values of a row as they are in memory.
+template <typename T, int EPL, bool VEC>
+struct alignas(VEC ? 16 : sizeof(T)) Raw {
+  T v[EPL];
+};
+template <typename T, int EPL, bool VEC>
+__device__ __forceinline__ void load_row(const BalanceArgs& a, int t, int lane, Raw<T, EPL, VEC>& r) {
   const T* row = static_cast<const T*>(a.logits) + t * a.stride;
-  float top = -INFINITY;
+  constexpr int kRun = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = i * 32 + lane;
-    s[i] = e < a.E ? to_f32<T>(row[e]) : -INFINITY;
-    top = s[i] > top || s[i] != s[i] ? s[i] : top;       // a NaN stays
+  for (int i = 0; i < EPL; i += kRun) {
+    const int e = expert_of<T, VEC>(i, lane);
+    if (e >= a.E) continue;
+    if (VEC) *reinterpret_cast<uint4*>(r.v + i) = *reinterpret_cast<const uint4*>(row + e);
+    else r.v[i] = row[e];
   }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    const float o = __shfl_xor_sync(0xFFFFFFFFu, top, d);
-    top = o > top || o != o ? o : top;
-  }
+}
+
+// Probabilities of a row, zero where the row has none, and (SLOPE) what dp/dz needs beside them: 1 - sigmoid(z) (1 for a
+// softmax), formed as e^-z sigmoid(z) where 1 - sigmoid(z) would cancel.
+template <typename T, int EPL, bool VEC, bool SLOPE>
+__device__ __forceinline__ void probabilities(const BalanceArgs& a, const Raw<T, EPL, VEC>& r, int lane, float (&p)[EPL], float (&slope)[EPL]) {
   float sum = 0.0f;
-  // sigmoid(z) is e^z to fp32 below -60, and would lose its bits below -87: such a row is shifted like a softmax's
-  const bool shifted = a.softmax || top < -60.0f;
+  if (!a.softmax) {
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const float z = s[i];
-    const float x = expf(shifted ? z - top : -z);
-    p[i] = shifted ? (z == -INFINITY ? 0.0f : x) : 1.0f / (1.0f + x);
-    s[i] = shifted ? 1.0f : z > 0.0f ? x * p[i] : 1.0f - p[i];
-    sum += p[i];
+    for (int i = 0; i < EPL; ++i) {
+      const float z = expert_of<T, VEC>(i, lane) < a.E ? to_f32<T>(r.v[i]) : -INFINITY;
+      const float x = expf(-z);
+      p[i] = __fdividef(1.0f, 1.0f + x);
+      if (x > 0x1p125f) p[i] = 0.0f;                     // beyond the fast division's range; the row is shifted if it matters
+      if (SLOPE) slope[i] = z > 0.0f ? x * p[i] : 1.0f - p[i];
+      sum += p[i];
+    }
+    sum = warp_sum(sum);
   }
-  sum = warp_sum(sum);
+  // sigmoid(z) is e^z to fp32 below -60 and loses its bits below -87: a row with nothing larger (or a NaN) is shifted by
+  // its largest value like a softmax's
+  if (a.softmax || !(sum > 0x1p-80f)) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      p[i] = expert_of<T, VEC>(i, lane) < a.E ? to_f32<T>(r.v[i]) : -INFINITY;
+      top = fmaxf(top, p[i]);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      p[i] = p[i] == -INFINITY ? 0.0f : expf(p[i] - top);
+      if (SLOPE) slope[i] = 1.0f;
+      sum += p[i];
+    }
+    sum = warp_sum(sum);
+  }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
   for (int i = 0; i < EPL; ++i) p[i] *= inv;
 }
 
-template <typename T, int EPL>
-__global__ void __launch_bounds__(32 * kChunkWarps) balance_chunk_kernel(BalanceArgs a) {
+// Tokens first, first + step, ... below end: adds their probabilities to acc and their selections to hist (shared
+// memory); returns how many counted.
+template <typename T, int EPL, bool VEC>
+__device__ __forceinline__ int add_tokens(const BalanceArgs& a, int first, int end, int step, int lane, float (&acc)[EPL], int* hist) {
+  int n = 0;
+  Raw<T, EPL, VEC> next;
+  int next_e = -1;                               // the lane's selection; more than 32 of them are read where they count
+  bool next_live = false;
+  auto fetch = [&](int t) {
+    next_live = t < end && (!a.mask || a.mask[t]);
+    if (!next_live) return;
+    load_row(a, t, lane, next);
+    if (lane < a.K) next_e = a.topk_idx[static_cast<int64_t>(t) * a.K + lane];
+  };
+  fetch(first);
+  for (int t = first; t < end; t += step) {
+    const Raw<T, EPL, VEC> now = next;
+    const int e = next_e;
+    const bool live = next_live;
+    fetch(t + step);
+    if (!live) continue;
+    if (e >= 0 && e < a.E) atomicAdd(hist + e, 1);
+    for (int k = lane + 32; k < a.K; k += 32) {
+      const int more = a.topk_idx[static_cast<int64_t>(t) * a.K + k];
+      if (more >= 0 && more < a.E) atomicAdd(hist + more, 1);
+    }
+    float p[EPL], none[EPL];
+    probabilities<T, EPL, VEC, false>(a, now, lane, p, none);
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) acc[i] += p[i];
+    ++n;
+  }
+  return n;
+}
+
+__device__ __forceinline__ float loss_of(const BalanceArgs& a, float dot, int n) {
+  return n ? a.alpha * a.E / a.K * (dot / n / n) : 0.0f;
+}
+
+template <typename T, int EPL, bool VEC>
+__global__ void __launch_bounds__(32 * chunk_warps(EPL)) balance_chunk_kernel(BalanceArgs a) {
+  constexpr int kChunkWarps = chunk_warps(EPL);
   griddep_launch_dependents();
   griddep_wait();
-  extern __shared__ float sh[];
-  float* sums = sh;                                              // [kChunkWarps][EPL * 32]
-  int* hist = reinterpret_cast<int*>(sh + kChunkWarps * EPL * 32);  // [EPL * 32]
+  extern __shared__ float sums[];                // [kChunkWarps][E]: sums of the warps, or a histogram for each
+  int* const hists = reinterpret_cast<int*>(sums);
+  int* const hist = hists + kChunkWarps * a.E;   // [E] of the whole CTA
   __shared__ float red[32];
-  __shared__ int n_valid;
+  __shared__ int n_valid, found[2];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x;
   const int t0 = c * a.chunk, t1 = min(a.T, t0 + a.chunk);
   const bool last = c == a.n_chunks - 1;
-  const int first = begun_before(a, t0, lane);
-  const int end = last ? a.S : begun_before(a, t1, lane);
+  if (w < 2) {
+    const int s = w == 0 ? begun_before(a, t0, lane) : last ? a.S : begun_before(a, t1, lane);
+    if (lane == 0) found[w] = s;
+  }
+  __syncthreads();
+  const int first = found[0], end = found[1];    // sequences that begin in the chunk
+
+  // short ones inside the chunk: a warp each
+  for (int q = first + w; q < end; q += kChunkWarps) {
+    const int b0 = border(a, q), b1 = max(border(a, q + 1), b0);
+    if (b1 > t1 || b1 - b0 > kShort) continue;
+    int* const mine = hists + w * a.E;
+    for (int e = lane; e < a.E; e += 32) mine[e] = 0;
+    __syncwarp();
+    float acc[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) acc[i] = 0.0f;
+    const int n = add_tokens<T, EPL, VEC>(a, b0, b1, 1, lane, acc, mine);
+    __syncwarp();
+    float dot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const int e = expert_of<T, VEC>(i, lane);
+      if (e < a.E) dot += static_cast<float>(mine[e]) * acc[i];
+    }
+    for (int e = lane; e < a.E; e += 32) a.counts[static_cast<int64_t>(q) * a.E + e] = mine[e];
+    dot = warp_sum(dot);
+    if (lane == 0) {
+      a.tokens[q] = n;
+      a.loss[q] = loss_of(a, dot, n);
+    }
+    __syncwarp();
+  }
+
+  // the others, all warps together; the first of them may have begun before the chunk
   int tail = -1;
   for (int q = first > 0 ? first - 1 : 0; q < end; ++q) {
     const int b0 = border(a, q), b1 = max(border(a, q + 1), b0);
     const bool head = q < first;
-    if (head && b1 <= t0) continue;
+    if (head ? b1 <= t0 : b1 <= t1 && b1 - b0 <= kShort) continue;
     const int lo = max(b0, t0), hi = min(b1, t1);
+    __syncthreads();
     for (int e = threadIdx.x; e < a.E; e += blockDim.x) hist[e] = 0;
     if (threadIdx.x == 0) n_valid = 0;
     __syncthreads();
     float acc[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; ++i) acc[i] = 0.0f;
-    int n = 0;
-    for (int t = lo + w; t < hi; t += kChunkWarps) {
-      if (a.mask && !a.mask[t]) continue;
-      float s[EPL], p[EPL];
-      probabilities<T, EPL>(a, t, lane, s, p);
+    const int n = add_tokens<T, EPL, VEC>(a, lo + w, hi, kChunkWarps, lane, acc, hist);
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) acc[i] += p[i];
-      for (int k = lane; k < a.K; k += 32) {
-        const int e = a.topk_idx[static_cast<int64_t>(t) * a.K + k];
-        if (e >= 0 && e < a.E) atomicAdd(hist + e, 1);
-      }
-      ++n;
+    for (int i = 0; i < EPL; ++i) {
+      const int e = expert_of<T, VEC>(i, lane);
+      if (e < a.E) sums[w * a.E + e] = acc[i];
     }
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) sums[(w * EPL + i) * 32 + lane] = acc[i];
     if (lane == 0) atomicAdd(&n_valid, n);
     __syncthreads();
     const bool whole = !head && b1 <= t1;
     const int slot = c * 2 + (head ? 0 : 1);
+    const int used = min(kChunkWarps, hi - lo);  // warps that had a token
     float dot[1] = {0.0f};
     for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
       float p = 0.0f;
-#pragma unroll
-      for (int v = 0; v < kChunkWarps; ++v) p += sums[v * EPL * 32 + e];
+#pragma unroll 8
+      for (int v = 0; v < used; ++v) p += sums[v * a.E + e];
       if (whole) {
         a.counts[static_cast<int64_t>(q) * a.E + e] = hist[e];
         dot[0] += static_cast<float>(hist[e]) * p;
@@ -155,63 +258,88 @@ __global__ void __launch_bounds__(32 * kChunkWarps) balance_chunk_kernel(Balance
     }
     if (whole) block_sum(dot, red);
     if (threadIdx.x == 0) {
-      const float n_all = static_cast<float>(n_valid);
       if (whole) {
         a.tokens[q] = n_valid;
-        a.loss[q] = n_valid ? a.alpha * a.E / a.K * (dot[0] / n_all / n_all) : 0.0f;
+        a.loss[q] = loss_of(a, dot[0], n_valid);
       } else {
         a.part_n[slot] = n_valid;
       }
     }
     if (!head && b1 > t1) tail = q;
-    __syncthreads();
   }
   if (threadIdx.x == 0) a.tail[c] = tail;
 }
 
-// CTA c finishes the sequence that begins in chunk c and goes on after it, if there is one.
+// CTA c finishes the sequence that begins in chunk c and goes on after it, if there is one.  Strips of the partial rows
+// are added side by side and joined in order.
 __global__ void __launch_bounds__(1024) balance_join_kernel(BalanceArgs a) {
   griddep_launch_dependents();
   griddep_wait();
-  __shared__ float red[32];
+  __shared__ float red[32], strip_p[1024];
+  __shared__ int strip_c[1024], n_all;
   const int c = blockIdx.x, q = a.tail[c];
   if (q < 0) return;
   const int last = (max(border(a, q + 1), 1) - 1) / a.chunk;
-  float dot[1] = {0.0f};
-  for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
-    float p = a.part_p[static_cast<int64_t>(2 * c + 1) * a.E + e];
-    int n = a.part_c[static_cast<int64_t>(2 * c + 1) * a.E + e];
-#pragma unroll 4
-    for (int k = c + 1; k <= last; ++k) {
-      p += a.part_p[static_cast<int64_t>(2 * k) * a.E + e];
-      n += a.part_c[static_cast<int64_t>(2 * k) * a.E + e];
+  const int padded = (a.E + 31) / 32 * 32, strips = 1024 / padded;
+  const int strip = threadIdx.x / padded, e = threadIdx.x - strip * padded;
+  if (threadIdx.x == 0) n_all = 0;
+  __syncthreads();
+  float p = 0.0f;
+  int n = 0;
+  if (strip < strips && e < a.E) {
+    const int per = (last - c + strips) / strips;                    // rows c .. last
+    const int k0 = c + strip * per, k1 = min(last + 1, k0 + per);
+#pragma unroll 8
+    for (int k = k0; k < k1; ++k) {
+      const int64_t at = static_cast<int64_t>(2 * k + (k == c ? 1 : 0)) * a.E + e;
+      p += a.part_p[at];
+      n += a.part_c[at];
     }
-    a.counts[static_cast<int64_t>(q) * a.E + e] = n;
-    dot[0] += static_cast<float>(n) * p;
+  }
+  strip_p[threadIdx.x] = p;
+  strip_c[threadIdx.x] = n;
+  for (int k = c + threadIdx.x; k <= last; k += blockDim.x) atomicAdd(&n_all, a.part_n[2 * k + (k == c ? 1 : 0)]);
+  __syncthreads();
+  float dot[1] = {0.0f};
+  if (threadIdx.x < a.E) {
+    p = 0.0f;
+    n = 0;
+    for (int s = 0; s < strips; ++s) {
+      p += strip_p[s * padded + threadIdx.x];
+      n += strip_c[s * padded + threadIdx.x];
+    }
+    a.counts[static_cast<int64_t>(q) * a.E + threadIdx.x] = n;
+    dot[0] = static_cast<float>(n) * p;
   }
   block_sum(dot, red);
   if (threadIdx.x == 0) {
-    int n = a.part_n[2 * c + 1];
-    for (int k = c + 1; k <= last; ++k) n += a.part_n[2 * k];
-    a.tokens[q] = n;
-    a.loss[q] = n ? a.alpha * a.E / a.K * (dot[0] / n / n) : 0.0f;
+    a.tokens[q] = n_all;
+    a.loss[q] = loss_of(a, dot[0], n_all);
   }
 }
 
-// One warp per token.  The counts enter less their mean K n / E (rounded: an exact integer difference), which leaves the
-// gradient as it is, because sum p = 1, and keeps its difference from cancelling when the counts are nearly even.
-template <typename T, int EPL>
-__global__ void __launch_bounds__(32 * kChunkWarps) balance_backward_kernel(BalanceArgs a) {
+// A warp takes consecutive tokens.  The counts enter less their mean K n / E (rounded: an exact integer difference),
+// which leaves the gradient as it is, because sum p = 1, and keeps its difference from cancelling when the counts are
+// nearly even.  Bound by HBM (logits in, gradient out) at many tokens.
+template <typename T, int EPL, bool VEC>
+__global__ void __launch_bounds__(32 * kBackWarps) balance_backward_kernel(BalanceArgs a) {
   griddep_launch_dependents();
   griddep_wait();
+  constexpr int kRun = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
   const int lane = threadIdx.x & 31;
-  const int warps = gridDim.x * kChunkWarps, warp = blockIdx.x * kChunkWarps + (threadIdx.x >> 5);
+  const int warps = gridDim.x * kBackWarps, warp = blockIdx.x * kBackWarps + (threadIdx.x >> 5);
   const int per = (a.T + warps - 1) / warps;
-  const int t0 = warp * per, t1 = min(a.T, t0 + per);
+  const int t0 = static_cast<int>(min(static_cast<int64_t>(warp) * per, static_cast<int64_t>(a.T))), t1 = min(a.T, t0 + per);
   int q = -1, b0 = 0, b1 = -1;       // sequence of the counts in registers and its borders
   float c[EPL], factor = 0.0f;
+  Raw<T, EPL, VEC> next;
+  bool next_live = false;
+  if (t0 < t1 && (next_live = !a.mask || a.mask[t0])) load_row(a, t0, lane, next);
   for (int t = t0; t < t1; ++t) {
-    if (t < b0 || t >= b1) {
+    const Raw<T, EPL, VEC> now = next;
+    const bool unmasked = next_live;
+    if (t + 1 < t1 && (next_live = !a.mask || a.mask[t + 1])) load_row(a, t + 1, lane, next);
+    if (unmasked && (t < b0 || t >= b1)) {
       q = begun_before(a, t + 1, lane) - 1;
       b0 = b1 = 0;
       if (q >= 0) {
@@ -224,55 +352,71 @@ __global__ void __launch_bounds__(32 * kChunkWarps) balance_backward_kernel(Bala
         factor = a.grad_loss[q] * (a.alpha * a.E / a.K) / n / n;
 #pragma unroll
         for (int i = 0; i < EPL; ++i) {
-          const int e = i * 32 + lane;
+          const int e = expert_of<T, VEC>(i, lane);
           c[i] = e < a.E ? static_cast<float>(a.counts[static_cast<int64_t>(q) * a.E + e] - mean) : 0.0f;
         }
       }
     }
     T* out = static_cast<T*>(a.grad) + static_cast<int64_t>(t) * a.E;
-    const bool live = t >= b0 && t < b1 && !(a.mask && !a.mask[t]);
-    float s[EPL], p[EPL];
-    float dot = 0.0f;
-    if (live) {
-      probabilities<T, EPL>(a, t, lane, s, p);
+    Raw<T, EPL, VEC> result;
+    if (unmasked && t >= b0 && t < b1) {
+      float p[EPL], slope[EPL];
+      float dot = 0.0f;
+      probabilities<T, EPL, VEC, true>(a, now, lane, p, slope);
 #pragma unroll
       for (int i = 0; i < EPL; ++i) dot += c[i] * p[i];
       dot = warp_sum(dot);
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) result.v[i] = from_f32<T>(factor * (p[i] * slope[i]) * (c[i] - dot));
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) result.v[i] = from_f32<T>(0.0f);
     }
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      const int e = i * 32 + lane;
-      if (e < a.E) out[e] = from_f32<T>(live ? factor * (p[i] * s[i]) * (c[i] - dot) : 0.0f);
+    for (int i = 0; i < EPL; i += kRun) {
+      const int e = expert_of<T, VEC>(i, lane);
+      if (e >= a.E) continue;
+      if (VEC) *reinterpret_cast<uint4*>(out + e) = *reinterpret_cast<const uint4*>(result.v + i);
+      else out[e] = result.v[i];
     }
   }
 }
 
-// Tokens of a chunk: a batch of up to kMinChunk stays whole; a longer one gives at most kMaxChunks chunks.
+// Tokens of a chunk: a batch of up to kMinChunk stays whole; a longer one gives at most one chunk per SM.
 int chunk_tokens(int T) {
-  const int least = (T + kMaxChunks - 1) / kMaxChunks;
+  const int least = (T + kNumSMs - 1) / kNumSMs;
   return least > kMinChunk ? least : kMinChunk;
 }
 int chunk_count(int T) { return T > 0 ? (T + chunk_tokens(T) - 1) / chunk_tokens(T) : 1; }
 
-template <typename T, int EPL>
+template <typename T, int EPL, bool VEC>
 cudaError_t launch_chunks(const BalanceArgs& a, bool backward, cudaStream_t stream) {
   if (backward) {
-    const int ctas = (a.T + kChunkWarps - 1) / kChunkWarps;
-    return launch_pdl(balance_backward_kernel<T, EPL>, dim3(ctas < 8 * kNumSMs ? ctas : 8 * kNumSMs), dim3(32 * kChunkWarps),
-                      0, stream, a);
+    const int ctas = (a.T + kBackWarps - 1) / kBackWarps;
+    return launch_pdl(balance_backward_kernel<T, EPL, VEC>, dim3(ctas < 8 * kNumSMs ? ctas : 8 * kNumSMs), dim3(32 * kBackWarps), 0,
+                      stream, a);
   }
-  const size_t smem = static_cast<size_t>(kChunkWarps + 1) * EPL * 32 * 4;
-  return launch_pdl(balance_chunk_kernel<T, EPL>, dim3(a.n_chunks), dim3(32 * kChunkWarps), smem, stream, a);
+  constexpr int kChunkWarps = chunk_warps(EPL);
+  const size_t smem = static_cast<size_t>(kChunkWarps + 1) * a.E * 4;
+  const cudaError_t e = cudaFuncSetAttribute(balance_chunk_kernel<T, EPL, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (kChunkWarps + 1) * EPL * 32 * 4);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(balance_chunk_kernel<T, EPL, VEC>, dim3(a.n_chunks), dim3(32 * kChunkWarps), smem, stream, a);
 }
 
 template <typename T>
 cudaError_t launch_chunks(const BalanceArgs& a, bool backward, cudaStream_t stream) {
+  constexpr int kRun = 16 / static_cast<int>(sizeof(T));
+  const bool vec = a.E % kRun == 0 && a.stride % kRun == 0 && aligned(a.logits, 16) && (!backward || aligned(a.grad, 16));
   const int per_lane = (a.E + 31) / 32;
-  if (per_lane <= 2) return launch_chunks<T, 2>(a, backward, stream);
-  if (per_lane <= 4) return launch_chunks<T, 4>(a, backward, stream);
-  if (per_lane <= 8) return launch_chunks<T, 8>(a, backward, stream);
-  if (per_lane <= 16) return launch_chunks<T, 16>(a, backward, stream);
-  return launch_chunks<T, 32>(a, backward, stream);
+  if (vec) {
+    if (per_lane <= 8) return launch_chunks<T, 8, true>(a, backward, stream);
+    if (per_lane <= 16) return launch_chunks<T, 16, true>(a, backward, stream);
+    return launch_chunks<T, 32, true>(a, backward, stream);
+  }
+  if (per_lane <= 2) return launch_chunks<T, 2, false>(a, backward, stream);
+  if (per_lane <= 8) return launch_chunks<T, 8, false>(a, backward, stream);
+  return launch_chunks<T, 32, false>(a, backward, stream);
 }
 
 cudaError_t launch_balance(const BalanceArgs& a, int dtype, bool backward, cudaStream_t stream) {
@@ -319,7 +463,7 @@ extern "C" int moe_fp8_block_scale_balance_loss(const void* logits, int64_t logi
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   cudaError_t e = launch_balance(a, dtype, false, stream);
   if (e == cudaSuccess && a.n_chunks > 1)
-    e = launch_pdl(balance_join_kernel, dim3(a.n_chunks - 1), dim3(E < 1024 ? (E + 31) / 32 * 32 : 1024), 0, stream, a);
+    e = launch_pdl(balance_join_kernel, dim3(a.n_chunks - 1), dim3(1024), 0, stream, a);
   return launch_status(e, a.n_chunks > 1 ? 2 : 1);
 }
 

@@ -781,7 +781,7 @@ extern "C" int moe_fp8_block_scale_block_norm(const void* x, int64_t x_stride, c
   }
   if (bad_common(a, dtype, param_f32) || !(eps > 0.0f)) return MOE_B200_EINVAL;
   if (T == 0) return MOE_B200_OK;
-  if (!x || !pre_weight || !h || !rstd || (y && !stream_out)) return MOE_B200_EINVAL;
+  if (!x || !pre_weight || !h || !rstd || !aligned(rstd, 8) || (y && !stream_out)) return MOE_B200_EINVAL;
   const bool vec = vector_rows(a, dtype);
   if (h_scale && (H % kBlock != 0 || !vec)) return MOE_B200_EINVAL;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
@@ -813,7 +813,7 @@ extern "C" int moe_fp8_block_scale_block_norm_backward(
   a.dx = grad_x; a.dy = grad_y;
   if (bad_common(a, dtype, param_f32)) return MOE_B200_EINVAL;
   if (T == 0) return MOE_B200_OK;
-  if (!x || !pre_weight || !rstd || !grad_h || !grad_x || !grad_pre_weight || (y && !grad_y) ||
+  if (!x || !pre_weight || !rstd || !aligned(rstd, 8) || !grad_h || !grad_x || !grad_pre_weight || (y && !grad_y) ||
       (post_weight && !grad_post_weight) || (gate_kind != kGateNone && !grad_gate) || !workspace || !aligned(workspace, 16))
     return MOE_B200_EINVAL;
   if (workspace_bytes < moe_fp8_block_scale_block_norm_backward_workspace_bytes(T, H)) return MOE_B200_EWORKSPACE;

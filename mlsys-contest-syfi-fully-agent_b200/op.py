@@ -252,22 +252,37 @@ NORM_MAX_WIDTH, BALANCE_MAX_EXPERTS, MATVEC_MAX_PAIRS, MATVEC_MAX_EXPERTS = 1638
 _scratch_bytes: Dict[tuple, int] = {}          # library's workspace size per kind and sizes
 
 
-def _scratch(kind, fn, a: int, b: int, dev: torch.device) -> torch.Tensor:
+def _scratch(kind, fn, a: int, b: int, like: torch.Tensor) -> torch.Tensor:
     need = _scratch_bytes.get((kind, a, b))
     if need is None:
         if len(_scratch_bytes) >= 4096:
             _scratch_bytes.clear()
         need = _scratch_bytes[kind, a, b] = int(fn(a, b))
-    return torch.empty(need, dtype=torch.uint8, device=dev)
+    return like.new_empty(need, dtype=torch.uint8)
 
 
-def _rows(name: str, t: torch.Tensor, T: int, H: int, dtype: torch.dtype, dev: torch.device):
+def _launch(fn, dev: torch.device, *args):
+    """Calls an entry point of the library with ``dev`` current and its stream as the last argument.  (A decode step's
+    kernel takes a few microseconds: the calls below spend as little host time as they can, so checks are written
+    without helpers that would format a message that is not needed.)"""
+    index = dev.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        loader.check(rc)
+
+
+def _rows(name: str, t: torch.Tensor, shape, dtype: torch.dtype, dev: torch.device):
     """Checks an activation argument [T, H] whose rows may lie apart; returns (address, row stride)."""
-    _check(t.dtype == dtype and t.dim() == 2 and t.shape[0] == T and t.shape[1] == H and t.device == dev,
-           f"{name} must be {dtype} [{T}, {H}] on {dev}")
+    if t.dtype is not dtype or t.shape != shape or t.device != dev:
+        raise ValueError(f"{name} must be {dtype} {list(shape)} on {dev}")
     stride = t.stride()
-    _check(stride[1] == 1 or H <= 1, f"{name}: the elements of a row must be adjacent")
-    return t.data_ptr(), stride[0] if T > 1 else 0
+    if stride[1] != 1 and shape[1] > 1:
+        raise ValueError(f"{name}: the elements of a row must be adjacent")
+    return t.data_ptr(), (stride[0] if shape[0] > 1 else 0)
 
 
 def _aligned(t: Optional[torch.Tensor]) -> bool:
@@ -277,45 +292,51 @@ def _aligned(t: Optional[torch.Tensor]) -> bool:
 
 
 def _on_gpu(t: torch.Tensor):
-    _check(t.is_cuda, "the tensors must be on a GPU: there is no CPU path")
+    if not t.is_cuda:
+        raise ValueError("the tensors must be on a GPU: there is no CPU path")
 
 
 def _param(name: str, t: torch.Tensor, H: int, dtype: torch.dtype, dev: torch.device):
     """Checks a parameter [H] in the activations' type or float32; returns (address, is float32)."""
-    _check((t.dtype == dtype or t.dtype == torch.float32) and t.dim() == 1 and t.shape[0] == H and
-           t.device == dev and (H <= 1 or t.stride(0) == 1), f"{name} must be a contiguous {dtype} or float32 [{H}] on {dev}")
-    return t.data_ptr(), t.dtype == torch.float32
+    f32 = t.dtype is torch.float32
+    if not (f32 or t.dtype is dtype) or t.dim() != 1 or t.shape[0] != H or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} or float32 [{H}] on {dev}")
+    return t.data_ptr(), f32
 
 
 def _norm_inputs(x, pre_weight, y, post_weight, gate, residual_scale):
     """Checks what both directions of the block norm take; returns the leading arguments of the C call."""
-    code = _TYPE_CODE.get(x.dtype)
-    _check(code is not None and x.dim() == 2, "x must be float32, bfloat16 or float16 [T, H]")
-    T, H = x.shape
-    _check(1 <= H <= NORM_MAX_WIDTH and T < 2 ** 31, f"x must have 1 to {NORM_MAX_WIDTH} columns")
-    dtype, dev = x.dtype, x.device
-    xp, xs = _rows("x", x, T, H, dtype, dev)
+    dtype, shape, dev = x.dtype, x.shape, x.device
+    code = _TYPE_CODE.get(dtype)
+    if code is None or len(shape) != 2:
+        raise ValueError("x must be float32, bfloat16 or float16 [T, H]")
+    T, H = shape
+    if not 1 <= H <= NORM_MAX_WIDTH or T >= 2 ** 31:
+        raise ValueError(f"x must have 1 to {NORM_MAX_WIDTH} columns")
+    xp, xs = _rows("x", x, shape, dtype, dev)
     pre, f32 = _param("pre_weight", pre_weight, H, dtype, dev)
     params = 1 if f32 else 0
-    yp = ys = post = gp = gs = kind = 0
+    yp = post = gp = None
+    ys = gs = kind = 0
     if y is not None:
-        yp, ys = _rows("y", y, T, H, dtype, dev)
+        yp, ys = _rows("y", y, shape, dtype, dev)
         if post_weight is not None:
             post, f32 = _param("post_weight", post_weight, H, dtype, dev)
-            params |= 2 if f32 else 0
+            if f32:
+                params |= 2
         if gate is not None:
             if gate.dim() == 1:
                 gp, f32 = _param("gate", gate, H, dtype, dev)
                 kind = 1
             else:
-                f32 = gate.dtype == torch.float32
-                per_token = gate.dim() == 2 and gate.shape[1] == 1
-                gp, gs = _rows("gate", gate, T, 1 if per_token else H, torch.float32 if f32 else dtype, dev)
-                kind = 2 if per_token else 3
-            params |= 4 if f32 else 0
-    else:
-        _check(post_weight is None and gate is None, "post_weight and gate belong to y")
-    return T, H, (xp, xs, yp or None, ys, gp or None, gs, kind, pre, post or None, T, H, code, params, float(residual_scale))
+                f32 = gate.dtype is torch.float32
+                kind = 2 if gate.dim() == 2 and gate.shape[1] == 1 else 3
+                gp, gs = _rows("gate", gate, (T, 1) if kind == 2 else shape, torch.float32 if f32 else dtype, dev)
+            if f32:
+                params |= 4
+    elif post_weight is not None or gate is not None:
+        raise ValueError("post_weight and gate belong to y")
+    return T, H, (xp, xs, yp, ys, gp, gs, kind, pre, post, T, H, code, params, float(residual_scale))
 
 
 def block_norm(x: torch.Tensor, pre_weight: torch.Tensor, y: Optional[torch.Tensor] = None,
@@ -333,29 +354,26 @@ def block_norm(x: torch.Tensor, pre_weight: torch.Tensor, y: Optional[torch.Tens
     [H / 128, T]) that ``run`` takes as hidden_states and hidden_states_scale, rounded from the unrounded h; H must then
     be a multiple of 128 and all rows 16-byte aligned.  Arithmetic is float32, what is stored is rounded once."""
     T, H, args = _norm_inputs(x, pre_weight, y, post_weight, gate, residual_scale)
-    _check(eps > 0.0, "eps must be positive")
+    if not eps > 0.0:
+        raise ValueError("eps must be positive")
     if quantize:
-        _check(H % BLOCK == 0, f"quantize needs a multiple of {BLOCK} columns")
-        per_token = gate is not None and gate.dim() == 2 and gate.shape[1] == 1
-        _check(_aligned(x) and _aligned(y) and _aligned(pre_weight) and _aligned(post_weight) and
-               (per_token or _aligned(gate)), "quantize needs rows that are 16-byte aligned")
+        if H % BLOCK != 0:
+            raise ValueError(f"quantize needs a multiple of {BLOCK} columns")
+        if not (_aligned(x) and _aligned(y) and _aligned(pre_weight) and _aligned(post_weight) and
+                (args[6] == 2 or _aligned(gate))):
+            raise ValueError("quantize needs rows that are 16-byte aligned")
     _on_gpu(x)
-    dev = x.device
-    s = x if y is None else torch.empty((T, H), dtype=x.dtype, device=dev)
-    rstd = torch.empty((T, 2), dtype=torch.float32, device=dev)
+    s = x if y is None else x.new_empty((T, H))
+    rstd = x.new_empty((T, 2), dtype=torch.float32)
     scale = None
     if quantize:
-        h = torch.empty((T, H), dtype=torch.float8_e4m3fn, device=dev)
-        scale = torch.empty((H // BLOCK, T), dtype=torch.float32, device=dev)
+        h = x.new_empty((T, H), dtype=torch.float8_e4m3fn)
+        scale = x.new_empty((H // BLOCK, T), dtype=torch.float32)
     else:
-        h = torch.empty((T, H), dtype=x.dtype, device=dev)
+        h = x.new_empty((T, H))
     if T:
-        with _on_device(dev):
-            rc = loader.lib.moe_fp8_block_scale_block_norm(
-                *args, eps, None if y is None else s.data_ptr(), h.data_ptr(), scale.data_ptr() if quantize else None,
-                rstd.data_ptr(), _stream_of(dev))
-        if rc:
-            loader.check(rc)
+        _launch(loader.lib.moe_fp8_block_scale_block_norm, x.device, *args, eps, None if y is None else s.data_ptr(),
+                h.data_ptr(), scale.data_ptr() if quantize else None, rstd.data_ptr())
     return s, ((h, scale) if quantize else h), rstd
 
 
@@ -368,49 +386,54 @@ def block_norm_backward(x: torch.Tensor, pre_weight: torch.Tensor, rstd: torch.T
     gradients of ``x``, ``y``, ``gate``, ``pre_weight`` and ``post_weight`` in their shapes and types, None where there
     is no such argument.  Sums over tokens are float32 in a fixed order."""
     T, H, args = _norm_inputs(x, pre_weight, y, post_weight, gate, residual_scale)
-    dev, dtype = x.device, x.dtype
-    _check(rstd.dtype == torch.float32 and tuple(rstd.shape) == (T, 2) and rstd.is_contiguous() and rstd.device == dev,
-           "rstd must be the float32 [T, 2] that block_norm returned")
-    gh = _rows("grad_h", grad_h, T, H, dtype, dev)
-    gs = (None, 0) if grad_stream is None else _rows("grad_stream", grad_stream, T, H, dtype, dev)
+    dev, dtype, shape = x.device, x.dtype, x.shape
+    if rstd.dtype is not torch.float32 or rstd.shape != (T, 2) or not rstd.is_contiguous() or rstd.device != dev or \
+            rstd.data_ptr() % 8 != 0:
+        raise ValueError("rstd must be the float32 [T, 2] that block_norm returned")
+    gh, gh_stride = _rows("grad_h", grad_h, shape, dtype, dev)
+    gs, gs_stride = (None, 0) if grad_stream is None else _rows("grad_stream", grad_stream, shape, dtype, dev)
     _on_gpu(x)
-    new = torch.empty if T else torch.zeros        # no token: the sums over tokens are zero
-    out = {"x": torch.empty((T, H), dtype=dtype, device=dev),
-           "pre_weight": new(H, dtype=pre_weight.dtype, device=dev),
-           "y": None if y is None else torch.empty((T, H), dtype=dtype, device=dev),
-           "post_weight": None if post_weight is None else new(H, dtype=post_weight.dtype, device=dev),
-           "gate": None if gate is None else new(gate.shape, dtype=gate.dtype, device=dev)}
-    if T:
-        ws = _scratch("norm", loader.lib.moe_fp8_block_scale_block_norm_backward_workspace_bytes, T, H, dev)
-        ptr = {k: None if v is None else v.data_ptr() for k, v in out.items()}
-        with _on_device(dev):
-            rc = loader.lib.moe_fp8_block_scale_block_norm_backward(
-                *args, rstd.data_ptr(), *gh, *gs, ptr["x"], ptr["y"], ptr["gate"], ptr["pre_weight"],
-                ptr["post_weight"], ws.data_ptr(), ws.numel(), _stream_of(dev))
-        if rc:
-            loader.check(rc)
+    out = {"x": x.new_empty((T, H)), "pre_weight": torch.empty_like(pre_weight),
+           "y": None if y is None else x.new_empty((T, H)),
+           "post_weight": None if post_weight is None else torch.empty_like(post_weight),
+           "gate": None if gate is None else gate.new_empty(gate.shape)}
+    if T == 0:                                     # the sums over no token
+        for k in ("pre_weight", "post_weight", "gate"):
+            if out[k] is not None:
+                out[k].zero_()
+        return out
+    ws = _scratch("norm", loader.lib.moe_fp8_block_scale_block_norm_backward_workspace_bytes, T, H, x)
+    _launch(loader.lib.moe_fp8_block_scale_block_norm_backward, dev, *args, rstd.data_ptr(), gh, gh_stride, gs, gs_stride,
+            *[None if out[k] is None else out[k].data_ptr() for k in ("x", "y", "gate", "pre_weight", "post_weight")],
+            ws.data_ptr(), ws.shape[0])
     return out
 
 
 def _balance_inputs(logits, top_k, cu_seqlens, token_mask, scoring):
     """Checks what both directions of the balance loss take; returns (type code, T, E, S, arguments after K)."""
+    shape, dev = logits.shape, logits.device
     code = _TYPE_CODE.get(logits.dtype)
-    _check(code is not None and logits.dim() == 2, "logits must be float32, bfloat16 or float16 [T, E]")
-    T, E = logits.shape
-    dev = logits.device
-    _check(1 <= E <= BALANCE_MAX_EXPERTS and T < 2 ** 31, f"logits must have 1 to {BALANCE_MAX_EXPERTS} columns")
-    _check(E == 1 or logits.stride(1) == 1, "logits: the elements of a row must be adjacent")
-    _check(1 <= top_k <= E, "every token selects 1 to E experts")
-    _check(scoring in _SCORING, "scoring must be 'sigmoid' or 'softmax'")
-    S, cu = 1, None
+    if code is None or len(shape) != 2:
+        raise ValueError("logits must be float32, bfloat16 or float16 [T, E]")
+    T, E = shape
+    if not 1 <= E <= BALANCE_MAX_EXPERTS or T >= 2 ** 31:
+        raise ValueError(f"logits must have 1 to {BALANCE_MAX_EXPERTS} columns")
+    if E > 1 and logits.stride(1) != 1:
+        raise ValueError("logits: the elements of a row must be adjacent")
+    if not 1 <= top_k <= E:
+        raise ValueError("every token selects 1 to E experts")
+    if scoring not in _SCORING:
+        raise ValueError("scoring must be 'sigmoid' or 'softmax'")
+    S, cu, mask = 1, None, None
     if cu_seqlens is not None:
-        _check(cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1 and
-               cu_seqlens.is_contiguous() and cu_seqlens.device == dev, f"cu_seqlens must be int32 [sequences + 1] on {dev}")
+        if cu_seqlens.dtype is not torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or \
+                not cu_seqlens.is_contiguous() or cu_seqlens.device != dev:
+            raise ValueError(f"cu_seqlens must be a contiguous int32 [sequences + 1] on {dev}")
         S, cu = cu_seqlens.shape[0] - 1, cu_seqlens.data_ptr()
-    mask = None
     if token_mask is not None:
-        _check(token_mask.dtype == torch.bool and tuple(token_mask.shape) == (T,) and token_mask.is_contiguous() and
-               token_mask.device == dev, f"token_mask must be bool [{T}] on {dev}")
+        if token_mask.dtype is not torch.bool or token_mask.shape != (T,) or not token_mask.is_contiguous() or \
+                token_mask.device != dev:
+            raise ValueError(f"token_mask must be a contiguous bool [{T}] on {dev}")
         mask = token_mask.data_ptr() or None
     return code, T, E, S, (cu, S, mask, _SCORING[scoring])
 
@@ -426,23 +449,22 @@ def balance_loss(logits: torch.Tensor, topk_idx: torch.Tensor, alpha: float, cu_
     count nowhere).  cu_seqlens int32 [S + 1] has the ascending borders of packed sequences (tokens outside every
     sequence are left out; None: one sequence); tokens with a False in token_mask [T] are left out too, whatever their
     rows hold.  Returns (loss float32 [S], counts int32 [S, E], tokens int32 [S]); a sequence without a token has loss 0."""
-    _check(topk_idx.dtype == torch.int32 and topk_idx.dim() == 2 and topk_idx.is_contiguous() and
-           topk_idx.device == logits.device, "topk_idx must be a contiguous int32 [T, K] on the logits' device")
-    code, T, E, S, rest = _balance_inputs(logits, topk_idx.shape[1], cu_seqlens, token_mask, scoring)
-    _check(topk_idx.shape[0] == T, "topk_idx must have a row for every token")
+    if topk_idx.dtype is not torch.int32 or topk_idx.dim() != 2 or not topk_idx.is_contiguous() or \
+            topk_idx.device != logits.device:
+        raise ValueError("topk_idx must be a contiguous int32 [T, K] on the logits' device")
+    rows, K = topk_idx.shape
+    code, T, E, S, rest = _balance_inputs(logits, K, cu_seqlens, token_mask, scoring)
+    if rows != T:
+        raise ValueError("topk_idx must have a row for every token")
     _on_gpu(logits)
-    dev = logits.device
-    loss = torch.empty(S, dtype=torch.float32, device=dev)
-    counts = torch.empty((S, E), dtype=torch.int32, device=dev)
-    tokens = torch.empty(S, dtype=torch.int32, device=dev)
+    loss = logits.new_empty(S, dtype=torch.float32)
+    counts = topk_idx.new_empty((S, E))
+    tokens = topk_idx.new_empty(S)
     if S:
-        ws = _scratch("balance", loader.lib.moe_fp8_block_scale_balance_loss_workspace_bytes, T, E, dev)
-        with _on_device(dev):
-            rc = loader.lib.moe_fp8_block_scale_balance_loss(
-                logits.data_ptr(), logits.stride(0), code, topk_idx.data_ptr(), T, E, topk_idx.shape[1], *rest, float(alpha),
-                loss.data_ptr(), counts.data_ptr(), tokens.data_ptr(), ws.data_ptr(), ws.numel(), _stream_of(dev))
-        if rc:
-            loader.check(rc)
+        ws = _scratch("balance", loader.lib.moe_fp8_block_scale_balance_loss_workspace_bytes, T, E, logits)
+        _launch(loader.lib.moe_fp8_block_scale_balance_loss, logits.device, logits.data_ptr(), logits.stride(0), code,
+                topk_idx.data_ptr(), T, E, K, *rest, float(alpha), loss.data_ptr(), counts.data_ptr(), tokens.data_ptr(),
+                ws.data_ptr(), ws.shape[0])
     return loss, counts, tokens
 
 
@@ -453,21 +475,17 @@ def balance_loss_backward(grad_loss: torch.Tensor, logits: torch.Tensor, counts:
     counts and tokens it returned; the counts are constants.  Rows of tokens that were left out are zero."""
     code, T, E, S, rest = _balance_inputs(logits, top_k, cu_seqlens, token_mask, scoring)
     dev = logits.device
-    _check(grad_loss.dtype == torch.float32 and tuple(grad_loss.shape) == (S,) and grad_loss.is_contiguous() and
-           grad_loss.device == dev, f"grad_loss must be a contiguous float32 [{S}] on {dev}")
-    _check(counts.dtype == torch.int32 and tuple(counts.shape) == (S, E) and counts.is_contiguous() and
-           counts.device == dev, f"counts must be a contiguous int32 [{S}, {E}] on {dev}")
-    _check(tokens.dtype == torch.int32 and tuple(tokens.shape) == (S,) and tokens.is_contiguous() and
-           tokens.device == dev, f"tokens must be a contiguous int32 [{S}] on {dev}")
+    if grad_loss.dtype is not torch.float32 or grad_loss.shape != (S,) or not grad_loss.is_contiguous() or grad_loss.device != dev:
+        raise ValueError(f"grad_loss must be a contiguous float32 [{S}] on {dev}")
+    if counts.dtype is not torch.int32 or counts.shape != (S, E) or not counts.is_contiguous() or counts.device != dev:
+        raise ValueError(f"counts must be a contiguous int32 [{S}, {E}] on {dev}")
+    if tokens.dtype is not torch.int32 or tokens.shape != (S,) or not tokens.is_contiguous() or tokens.device != dev:
+        raise ValueError(f"tokens must be a contiguous int32 [{S}] on {dev}")
     _on_gpu(logits)
-    grad = torch.empty((T, E), dtype=logits.dtype, device=dev)
+    grad = logits.new_empty((T, E))
     if T:
-        with _on_device(dev):
-            rc = loader.lib.moe_fp8_block_scale_balance_loss_backward(
-                grad_loss.data_ptr(), logits.data_ptr(), logits.stride(0), code, counts.data_ptr(), tokens.data_ptr(),
-                T, E, top_k, *rest, float(alpha), grad.data_ptr(), _stream_of(dev))
-        if rc:
-            loader.check(rc)
+        _launch(loader.lib.moe_fp8_block_scale_balance_loss_backward, dev, grad_loss.data_ptr(), logits.data_ptr(),
+                logits.stride(0), code, counts.data_ptr(), tokens.data_ptr(), T, E, top_k, *rest, float(alpha), grad.data_ptr())
     return grad
 
 
@@ -477,50 +495,56 @@ def matvec_w4(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor, zero:
 
         out[r, n] = sum_k x[r, k] * (q[n, k] - zero[n, k // G]) * scale[n, k // G]
 
-    x bfloat16 / float16 [R, K]; qweight uint8 [N, K / 2], two values a byte, the even k in the low half; scale
-    [N, K / G] in x's type or float32, G = 32, 64 or 128; zero uint8 [N, K / G] (None: 8).  With ``experts`` the weights
-    have a leading dimension E and every (row, choice) has its own matrix: experts int32 [R] gives out [R, N], [R, k]
-    gives [R, k, N] (the experts that ``route`` selected, less the shard's first); an expert outside [0, E) gives zeros.
-    At most 256 (row, choice) pairs and 1024 experts.  out has x's type, or float32 with ``out_dtype``; sums are float32."""
-    code = _TYPE_CODE.get(x.dtype) if x.dtype != torch.float32 else None
-    _check(code is not None and x.dim() == 2, "x must be bfloat16 or float16 [R, K]")
-    R, K = x.shape
-    dev = x.device
+    x bfloat16 / float16 [R, K] (bfloat16: |x| < 2^63); qweight uint8 [N, K / 2], two values a byte, the even k in the
+    low half; scale [N, K / G] in x's type or float32, G = 32, 64 or 128; zero uint8 [N, K / G], 0 to 15 (None: 8).  With
+    ``experts`` the weights have a leading dimension E and every (row, choice) has its own matrix: experts int32 [R] gives
+    out [R, N], [R, k] gives [R, k, N] (the experts that ``route`` selected, less the shard's first); an expert outside
+    [0, E) gives zeros.  At most 256 (row, choice) pairs and 1024 experts.  out has x's type, or float32 with
+    ``out_dtype``; sums are float32."""
+    dtype, dev, shape = x.dtype, x.device, x.shape
+    if (dtype is not torch.bfloat16 and dtype is not torch.float16) or len(shape) != 2:
+        raise ValueError("x must be bfloat16 or float16 [R, K]")
+    R, K = shape
     lead = 0 if experts is None else 1
-    _check(qweight.dtype == torch.uint8 and qweight.dim() == 2 + lead and qweight.is_contiguous() and
-           qweight.device == dev and K >= 1 and qweight.shape[-1] * 2 == K and qweight.numel() > 0,
-           f"qweight must be a contiguous uint8 [{'E, ' if lead else ''}N, {K} / 2] on {dev}")
-    E, N = (qweight.shape[0] if lead else 1), qweight.shape[-2]
-    _check(N <= 2 ** 22 and K <= 2 ** 20, "at most 2^22 rows and 2^20 columns")
-    groups = scale.shape[-1] if scale.dim() else 0
+    wshape = qweight.shape
+    if qweight.dtype is not torch.uint8 or len(wshape) != 2 + lead or not qweight.is_contiguous() or \
+            qweight.device != dev or K < 1 or wshape[-1] * 2 != K or qweight.numel() == 0:
+        raise ValueError(f"qweight must be a contiguous uint8 [{'E, ' if lead else ''}N, {K} / 2] on {dev}")
+    E, N = (wshape[0] if lead else 1), wshape[-2]
+    if N > 2 ** 22 or K > 2 ** 20 or E > MATVEC_MAX_EXPERTS:
+        raise ValueError(f"at most 2^22 rows, 2^20 columns and {MATVEC_MAX_EXPERTS} experts")
+    sshape, stype = scale.shape, scale.dtype
+    groups = sshape[-1] if len(sshape) else 0
     G = K // groups if groups else 0
-    _check(G in (32, 64, 128) and G * groups == K and (scale.dtype == x.dtype or scale.dtype == torch.float32) and
-           scale.shape[:-1] == qweight.shape[:-1] and scale.is_contiguous() and scale.device == dev,
-           f"scale must be a contiguous {x.dtype} or float32 [{'E, ' if lead else ''}N, K / G] on {dev}, G = 32, 64 or 128")
-    _check(zero is None or (zero.dtype == torch.uint8 and zero.shape == scale.shape and zero.is_contiguous() and
-                            zero.device == dev), "zero must be a contiguous uint8 tensor of scale's shape")
-    stride = x.stride()
-    _check((K == 1 or stride[1] == 1) and (R <= 1 or stride[0] % 8 == 0) and x.data_ptr() % 16 == 0,
-           "the rows of x must be 16-byte aligned and their elements adjacent")
-    per_row, shape, ids = 1, (R, N), None
+    if G not in (32, 64, 128) or G * groups != K or (stype is not dtype and stype is not torch.float32) or \
+            sshape[:-1] != wshape[:-1] or not scale.is_contiguous() or scale.device != dev:
+        raise ValueError(f"scale must be a contiguous {dtype} or float32 [{'E, ' if lead else ''}N, K / G] on {dev}, "
+                         "G = 32, 64 or 128")
+    if zero is not None and (zero.dtype is not torch.uint8 or zero.shape != sshape or not zero.is_contiguous() or
+                             zero.device != dev):
+        raise ValueError("zero must be a contiguous uint8 tensor of scale's shape")
+    stride, xp, qp = x.stride(), x.data_ptr(), qweight.data_ptr()
+    if (K > 1 and stride[1] != 1) or (R > 1 and stride[0] % 8 != 0) or xp % 16 != 0 or qp % 16 != 0:
+        raise ValueError("the rows of x and qweight must be 16-byte aligned and x's elements adjacent")
+    per_row, oshape, ids = 1, (R, N), None
     if lead:
-        _check(E <= MATVEC_MAX_EXPERTS, f"at most {MATVEC_MAX_EXPERTS} experts")
-        _check(experts.dtype == torch.int32 and experts.dim() in (1, 2) and experts.shape[0] == R and
-               experts.is_contiguous() and experts.device == dev, f"experts must be a contiguous int32 [{R}] or [{R}, k] on {dev}")
-        per_row = experts.shape[1] if experts.dim() == 2 else 1
-        shape, ids = tuple(experts.shape) + (N,), experts.data_ptr()
-    _check(R * per_row <= MATVEC_MAX_PAIRS, f"at most {MATVEC_MAX_PAIRS} (row, expert) pairs")
-    _check(out_dtype is None or out_dtype == x.dtype or out_dtype == torch.float32, "out_dtype must be x's type or float32")
+        eshape = experts.shape
+        if experts.dtype is not torch.int32 or len(eshape) not in (1, 2) or eshape[0] != R or \
+                not experts.is_contiguous() or experts.device != dev:
+            raise ValueError(f"experts must be a contiguous int32 [{R}] or [{R}, k] on {dev}")
+        per_row = eshape[1] if len(eshape) == 2 else 1
+        oshape, ids = (*eshape, N), experts.data_ptr()
+    pairs = R * per_row
+    if pairs > MATVEC_MAX_PAIRS:
+        raise ValueError(f"at most {MATVEC_MAX_PAIRS} (row, expert) pairs")
+    if out_dtype is not None and out_dtype is not dtype and out_dtype is not torch.float32:
+        raise ValueError("out_dtype must be x's type or float32")
     _on_gpu(x)
-    out = torch.empty(shape, dtype=out_dtype or x.dtype, device=dev)
-    if R * per_row:
-        with _on_device(dev):
-            rc = loader.lib.moe_fp8_block_scale_matvec_w4(
-                x.data_ptr(), stride[0], code, qweight.data_ptr(), scale.data_ptr(), scale.dtype == torch.float32,
-                None if zero is None else zero.data_ptr(), ids, R * per_row, per_row, E, N, K, G, out.data_ptr(),
-                out.dtype == torch.float32, _stream_of(dev))
-        if rc:
-            loader.check(rc)
+    out = x.new_empty(oshape, dtype=out_dtype)
+    if pairs:
+        _launch(loader.lib.moe_fp8_block_scale_matvec_w4, dev, xp, stride[0] if R > 1 else 0, _TYPE_CODE[dtype], qp,
+                scale.data_ptr(), stype is torch.float32, None if zero is None else zero.data_ptr(), ids, pairs, per_row, E, N,
+                K, G, out.data_ptr(), out_dtype is torch.float32)
     return out
 
 

@@ -109,6 +109,7 @@ def matvec_args(R=4, N=8, K=256, G=64, E=3):
     (dict(experts=torch.zeros(4, 2, dtype=torch.int64)), "experts"),
     (dict(experts=torch.zeros(5, dtype=torch.int32)), "experts"),
     (dict(experts=torch.zeros(4, 65, dtype=torch.int32)), "256"),
+    (dict(qweight=torch.zeros(3, 8, 129, dtype=torch.uint8).view(-1)[8:8 + 3 * 8 * 128].view(3, 8, 128)), "aligned"),
     (dict(out_dtype=torch.float16), "out_dtype"),
     (dict(experts=None), "qweight"),
     (dict(), "on a GPU"),
