@@ -157,18 +157,33 @@ __device__ __forceinline__ void clear_ring_ends(uint8_t* ring, uint32_t stage_by
   }
 }
 
-// Where the rows of the kernels without a ring come from: memory.  VEC rows come through the ring.
-template <typename T, int CH, bool VEC>
-__device__ __forceinline__ void row8(const uint8_t* stage, int array, const void* p, int64_t row_offset, int c, int H, F2 (&v)[4]) {
-  if (VEC) take8<T, CH>(stage, array, c, v);
-  else load8<T, false>(static_cast<const T*>(p) + row_offset, c, H, v);
+// Rows that do not start on 16 bytes (an odd width or stride, a view) go through the ring as the aligned blocks that cover
+// them; the last one brings only the row's bytes, so that nothing behind the row is read, and the bytes in front of the
+// row lie in the same 16 bytes of the same allocation.  The columns a thread takes are then blockDim.x apart, not what it
+// copied itself: these kernels have a barrier after the wait.
+__host__ __device__ constexpr int span_bytes(int H, int size) { return (H * size + 15) / 16 * 16 + 16; }
+
+template <typename T>
+__device__ __forceinline__ void fetch_span(uint32_t to, const T* row, int H) {
+  const uintptr_t from = reinterpret_cast<uintptr_t>(row) & ~uintptr_t(15);
+  const int bytes = static_cast<int>(reinterpret_cast<uintptr_t>(row) - from) + H * static_cast<int>(sizeof(T));
+  for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i), "l"(from + i), "r"(min(16, bytes - i)) : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ int row_low(const T* row) { return static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15); }
+
+template <typename T>
+__device__ __forceinline__ void take_span8(const uint8_t* row, int c, int H, F2 (&v)[4]) {
+  load8<T, false>(reinterpret_cast<const T*>(row), c, H, v);
 }
 
 // GATE: where the gate and the parameters' types are known (all of the activations' type), else kAnyGate.
 constexpr int kAnyGate = -1;
 
 template <typename T, int CH, bool VEC, bool QUANT, int GATE>
-__global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, !VEC ? 1 : CH == 1 ? 3 : CH == 2 ? 2 : 1) block_norm_kernel(NormArgs a) {
+__global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 3 : CH == 2 ? 2 : 1) block_norm_kernel(NormArgs a) {
   griddep_launch_dependents();
   griddep_wait();
   extern __shared__ __align__(16) uint8_t ring[];
@@ -178,7 +193,8 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, !VEC ? 1 : CH ==
   const float inv_h = 1.0f / static_cast<float>(H);
   // a full gate of another type than the activations' is read directly
   const bool full_in_ring = GATE == kGateFull || (GATE == kAnyGate && gate_kind == kGateFull && !(a.gate_f32 && sizeof(T) == 2));
-  const uint32_t stage_bytes = static_cast<uint32_t>(a.arrays * CH * blockDim.x * sizeof(Pack8<T>));
+  const int span = span_bytes(H, sizeof(T));
+  const uint32_t stage_bytes = static_cast<uint32_t>(a.arrays * (VEC ? CH * blockDim.x * sizeof(Pack8<T>) : span));
   auto param = [&](const void* p, int f32, int64_t offset, int c, F2 (&v)[4]) {
     if (GATE == kAnyGate) load8_param<T, VEC>(p, f32, offset, c, H, v);
     else load8<T, VEC>(static_cast<const T*>(p) + offset, c, H, v);
@@ -191,9 +207,15 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, !VEC ? 1 : CH ==
   const int64_t step = gridDim.x;
   auto fetch = [&](uint32_t stage) {
     if (fetch_at < a.T) {
-      fetch_row<T, CH>(stage, 0, fetch_x, H);
-      if (a.y) fetch_row<T, CH>(stage, 1, fetch_y, H);
-      if (full_in_ring) fetch_row<T, CH>(stage, 2, fetch_g, H);
+      if (VEC) {
+        fetch_row<T, CH>(stage, 0, fetch_x, H);
+        if (a.y) fetch_row<T, CH>(stage, 1, fetch_y, H);
+        if (full_in_ring) fetch_row<T, CH>(stage, 2, fetch_g, H);
+      } else {
+        fetch_span(stage, fetch_x, H);
+        if (a.y) fetch_span(stage + span, fetch_y, H);
+        if (full_in_ring) fetch_span(stage + 2 * span, fetch_g, H);
+      }
     }
     fetch_at += step;
     fetch_x += step * a.x_stride;
@@ -201,10 +223,14 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, !VEC ? 1 : CH ==
     fetch_g += step * a.gate_stride;
     copies_close();
   };
-  if (VEC) {
-    clear_ring_ends<T, CH>(ring, stage_bytes, a.ring, a.arrays, H);
-    for (int i = 0; i < a.ring; ++i) fetch(smem_address(ring) + i * stage_bytes);
-  }
+  // rows being worked on, for where they begin in their blocks
+  const T *row_x = fetch_x, *row_y = fetch_y, *row_g = fetch_g;
+  auto take = [&](const uint8_t* stage, int array, const T* from, int c, F2 (&v)[4]) {
+    if (VEC) take8<T, CH>(stage, array, c, v);
+    else take_span8<T>(stage + array * span + row_low(from), c, H, v);
+  };
+  if (VEC) clear_ring_ends<T, CH>(ring, stage_bytes, a.ring, a.arrays, H);
+  for (int i = 0; i < a.ring; ++i) fetch(smem_address(ring) + i * stage_bytes);
   T* s_out = static_cast<T*>(a.s) + blockIdx.x * static_cast<int64_t>(H);
   T* h_out = static_cast<T*>(a.h) + blockIdx.x * static_cast<int64_t>(H);
   uint8_t* q_out = a.q + blockIdx.x * static_cast<int64_t>(H);
@@ -215,17 +241,18 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, !VEC ? 1 : CH ==
     const uint8_t* const stage = ring + slot * stage_bytes;
     const float gate = next_gate;
     if (gate_kind == kGateToken && row + step < a.T) next_gate = token_gate<T>(a, row + step);
-    if (VEC) ring_wait(a.ring);
+    ring_wait(a.ring);
+    if (!VEC) __syncthreads();
     F2 s[CH][4];
     float r1 = 0.0f;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) row8<T, CH, VEC>(stage, 0, a.x, row * a.x_stride, c, H, s[c]);
+    for (int c = 0; c < CH; ++c) take(stage, 0, row_x, c, s[c]);
     if (a.y) {
       F2 n[CH][4];
       F2 g[4];
       float k = gate;                              // what a whole row of y is multiplied by
 #pragma unroll
-      for (int c = 0; c < CH; ++c) row8<T, CH, VEC>(stage, 1, a.y, row * a.y_stride, c, H, n[c]);
+      for (int c = 0; c < CH; ++c) take(stage, 1, row_y, c, n[c]);
       if (a.post_w) {
         F2 square = both(0.0f);
 #pragma unroll
@@ -246,7 +273,7 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, !VEC ? 1 : CH ==
       if (gate_kind == kGateChannel || gate_kind == kGateFull) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-          if (VEC && full_in_ring) take8<T, CH>(stage, 2, c, g);
+          if (full_in_ring) take(stage, 2, row_g, c, g);
           else param(a.gate, a.gate_f32, gate_kind == kGateFull ? row * a.gate_stride : 0, c, g);
 #pragma unroll
           for (int j = 0; j < 4; ++j) n[c][j] = mul2(n[c][j], g[j]);
@@ -260,10 +287,7 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, !VEC ? 1 : CH ==
         store8<T, VEC>(s_out, c, H, s[c]);
       }
     }
-    if (VEC) {
-      fetch(smem_address(stage));
-      slot = slot + 1 == a.ring ? 0 : slot + 1;
-    }
+    if (VEC) fetch(smem_address(stage));
     F2 square = both(0.0f);
 #pragma unroll
     for (int c = 0; c < CH; ++c)
@@ -271,6 +295,13 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, !VEC ? 1 : CH ==
       for (int j = 0; j < 4; ++j) square = fma2(s[c][j], s[c][j], square);
     float sum[1] = {total(square)};
     block_sum(sum, red[1]);
+    if (!VEC) {                                    // everybody has read the stage
+      fetch(smem_address(stage));
+      row_x += step * a.x_stride;
+      row_y += step * a.y_stride;
+      row_g += step * a.gate_stride;
+    }
+    slot = slot + 1 == a.ring ? 0 : slot + 1;
     const float r2 = rsqrtf(sum[0] * inv_h + a.eps);
     if (threadIdx.x == 0) *reinterpret_cast<float2*>(a.rstd + 2 * static_cast<int64_t>(row)) = make_float2(r1, r2);
     const F2 rr = both(r2);
@@ -308,7 +339,7 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, !VEC ? 1 : CH ==
     q_out += step_h;
     // red[0] of the next row is written only after every thread has passed the barrier of red[1], and without a first
     // sum red[1] would be written again while a slow thread reads it
-    if (!a.post_w) __syncthreads();
+    if (VEC && !a.post_w) __syncthreads();
   }
 }
 
@@ -435,44 +466,54 @@ __global__ void __launch_bounds__(kNormThreads) block_norm_backward_kernel(NormA
   }
 }
 
-// ... and this one where rows are aligned, parameters have the activations' type and a row fits 16 columns a thread: the
+// ... and this one where parameters have the activations' type and a row fits 16 columns a thread and the ring: the
 // rows come through a ring like the forward's, the column sums stay in registers as fp32, and the weights, which leave no
 // registers for themselves, in shared memory behind the ring (an SM's quarter has 128 registers for each of four warps).
 // Missing parts are neutral values (y = 0, w_post = 1, gate = 1) instead of branches.
-template <typename T, int CH, int MAXT, int GATE>
-__global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) block_norm_backward_ring_kernel(NormArgs a) {
+template <typename T, int CH, bool VEC, int GATE>
+__global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 2 : 1) block_norm_backward_ring_kernel(NormArgs a) {
   griddep_launch_dependents();
   griddep_wait();
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float red[2][96];
   const int H = a.H;
   const float inv_h = 1.0f / static_cast<float>(H), scale = a.y ? a.a : 1.0f;
-  const uint32_t stage_bytes = static_cast<uint32_t>(a.arrays * CH * blockDim.x * sizeof(Pack8<T>));
+  const int span = span_bytes(H, sizeof(T));
+  const uint32_t stage_bytes = static_cast<uint32_t>(a.arrays * (VEC ? CH * blockDim.x * sizeof(Pack8<T>) : span));
+  auto fetch_one = [&](uint32_t stage, int array, const void* p, int64_t at) {
+    if (VEC) fetch_row<T, CH>(stage, array, static_cast<const T*>(p) + at, H);
+    else fetch_span(stage + array * span, static_cast<const T*>(p) + at, H);
+  };
   // arrays of a stage: x, grad_h, grad_stream, y, gate; what the call lacks is never copied and stays zero
   auto fetch = [&](int64_t row, uint32_t stage) {
     if (row < a.T) {
-      fetch_row<T, CH>(stage, 0, static_cast<const T*>(a.x) + row * a.x_stride, H);
-      fetch_row<T, CH>(stage, 1, static_cast<const T*>(a.gh) + row * a.gh_stride, H);
-      if (a.gs) fetch_row<T, CH>(stage, 2, static_cast<const T*>(a.gs) + row * a.gs_stride, H);
-      if (a.y) fetch_row<T, CH>(stage, 3, static_cast<const T*>(a.y) + row * a.y_stride, H);
-      if (GATE == kGateFull) fetch_row<T, CH>(stage, 4, static_cast<const T*>(a.gate) + row * a.gate_stride, H);
+      fetch_one(stage, 0, a.x, row * a.x_stride);
+      fetch_one(stage, 1, a.gh, row * a.gh_stride);
+      if (a.gs) fetch_one(stage, 2, a.gs, row * a.gs_stride);
+      if (a.y) fetch_one(stage, 3, a.y, row * a.y_stride);
+      if (GATE == kGateFull) fetch_one(stage, 4, a.gate, row * a.gate_stride);
     }
     copies_close();
   };
   for (uint32_t i = threadIdx.x * 16; i < a.ring * stage_bytes; i += blockDim.x * 16) *reinterpret_cast<uint4*>(ring + i) = make_uint4(0u, 0u, 0u, 0u);
   __syncthreads();
-  for (int i = 0; i < a.ring; ++i) fetch(blockIdx.x + static_cast<int64_t>(i) * gridDim.x, smem_address(ring) + i * stage_bytes);
+  for (int i = 0; i < a.ring - (VEC ? 0 : 1); ++i) fetch(blockIdx.x + static_cast<int64_t>(i) * gridDim.x, smem_address(ring) + i * stage_bytes);
 
+  auto take = [&](const uint8_t* stage, int array, const void* p, int64_t at, int c, F2 (&v)[4]) {
+    if (VEC) take8<T, CH>(stage, array, c, v);
+    else if (p) take_span8<T>(stage + array * span + row_low(static_cast<const T*>(p) + at), c, H, v);
+    else v[0] = v[1] = v[2] = v[3] = both(0.0f);
+  };
   uint8_t* const weights = ring + a.ring * stage_bytes;    // w_pre, w_post, gate per channel: the thread's own pieces
   F2 sum_pre[CH][4], sum_post[CH][4], sum_gate[GATE == kGateChannel ? CH : 1][4];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const int col = column<true>(c, 0);
-    const F2 ones[4] = {both(1.0f), both(1.0f), both(1.0f), both(1.0f)};
     const void* const from[3] = {a.pre_w, a.post_w, GATE == kGateChannel ? a.gate : nullptr};
 #pragma unroll
     for (int k = 0; k < (GATE == kGateChannel ? 3 : 2); ++k) {
-      const Pack8<T> v = from[k] && col < H ? *reinterpret_cast<const Pack8<T>*>(static_cast<const T*>(from[k]) + col) : pack8<T>(ones);
+      F2 w[4] = {both(1.0f), both(1.0f), both(1.0f), both(1.0f)};
+      if (from[k]) load8<T, VEC>(static_cast<const T*>(from[k]), c, H, w);
+      const Pack8<T> v = pack8<T>(w);
 #pragma unroll
       for (int half = 0; half < static_cast<int>(sizeof(T)) / 2; ++half)
         *reinterpret_cast<uint4*>(weights + piece<T, CH>(k, c) + half * 16 * blockDim.x) = v.w[half];
@@ -500,20 +541,28 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) block_norm_backward
     const uint8_t* const stage = ring + slot * stage_bytes;
     const float r1 = next_r1, r2 = next_r2, gt = next_gt;
     stats(row + static_cast<int64_t>(gridDim.x), next_r1, next_r2, next_gt);
-    ring_wait(a.ring);
+    if (VEC) {
+      ring_wait(a.ring);
+    } else {
+      // the stage of the row before is free once all threads are here: a ring of n stages runs n - 1 rows ahead
+      if (a.ring == 3) copies_wait<1>();
+      else copies_wait<0>();
+      __syncthreads();
+      fetch(row + static_cast<int64_t>(a.ring - 1) * gridDim.x, smem_address(ring) + (slot == 0 ? a.ring - 1 : slot - 1) * stage_bytes);
+    }
     F2 sh[CH][4], d[CH][4];
     F2 dots[3] = {both(0.0f), both(0.0f), both(0.0f)};
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       F2 u[4], w[4], g[4], wp[4], yh[4];
-      take8<T, CH>(stage, 0, c, sh[c]);
-      take8<T, CH>(stage, 1, c, u);
-      take8<T, CH>(stage, 2, c, d[c]);
-      take8<T, CH>(stage, 3, c, yh);
+      take(stage, 0, a.x, row * a.x_stride, c, sh[c]);
+      take(stage, 1, a.gh, row * a.gh_stride, c, u);
+      take(stage, 2, a.gs, row * a.gs_stride, c, d[c]);
+      take(stage, 3, a.y, row * a.y_stride, c, yh);
       take8<T, CH>(weights, 0, c, w);
       take8<T, CH>(weights, 1, c, wp);
       if (GATE == kGateChannel) take8<T, CH>(weights, 2, c, g);
-      if (GATE == kGateFull) take8<T, CH>(stage, 4, c, g);
+      if (GATE == kGateFull) take(stage, 4, a.gate, row * a.gate_stride, c, g);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         F2 v = mul2(mul2(yh[j], both(r1)), wp[j]);
@@ -541,14 +590,14 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) block_norm_backward
         d[c][j] = fma2(both(-k2), sh[c][j], d[c][j]);
         out[j] = mul2(both(scale), d[c][j]);
       }
-      store8<T, true>(static_cast<T*>(a.dx) + static_cast<int64_t>(row) * H, c, H, out);
+      store8<T, VEC>(static_cast<T*>(a.dx) + static_cast<int64_t>(row) * H, c, H, out);
       if (!a.y) continue;
-      take8<T, CH>(stage, 3, c, yh);               // read again: registers are what this kernel is short of
+      take(stage, 3, a.y, row * a.y_stride, c, yh);               // read again: registers are what this kernel is short of
       take8<T, CH>(weights, 1, c, wp);
 #pragma unroll
       for (int j = 0; j < 4; ++j) yh[j] = mul2(yh[j], both(r1));
       if (GATE == kGateChannel) take8<T, CH>(weights, 2, c, g);
-      if (GATE == kGateFull) take8<T, CH>(stage, 4, c, g);
+      if (GATE == kGateFull) take(stage, 4, a.gate, row * a.gate_stride, c, g);
       if (GATE != kGateNone) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -556,7 +605,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) block_norm_backward
           if (GATE == kGateChannel) sum_gate[c][j] = fma2(d[c][j], n, sum_gate[c][j]);
           else out[j] = mul2(d[c][j], n);
         }
-        if (GATE == kGateFull) store8<T, true>(static_cast<T*>(a.dgate_rows) + static_cast<int64_t>(row) * H, c, H, out);
+        if (GATE == kGateFull) store8<T, VEC>(static_cast<T*>(a.dgate_rows) + static_cast<int64_t>(row) * H, c, H, out);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -564,17 +613,17 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) block_norm_backward
         sum_post[c][j] = fma2(dn, yh[j], sum_post[c][j]);
         out[j] = fma2(both(-k1), yh[j], mul2(mul2(dn, wp[j]), both(r1)));
       }
-      store8<T, true>(static_cast<T*>(a.dy) + static_cast<int64_t>(row) * H, c, H, out);
+      store8<T, VEC>(static_cast<T*>(a.dy) + static_cast<int64_t>(row) * H, c, H, out);
     }
-    fetch(row + static_cast<int64_t>(a.ring) * gridDim.x, smem_address(stage));
+    if (VEC) fetch(row + static_cast<int64_t>(a.ring) * gridDim.x, smem_address(stage));
     slot = slot + 1 == a.ring ? 0 : slot + 1;
   }
   float* dst = a.partial + static_cast<int64_t>(blockIdx.x) * a.n_sums * H;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    store8<float, true>(dst, c, H, sum_pre[c]);
-    if (a.sum_post >= 0) store8<float, true>(dst + static_cast<int64_t>(a.sum_post) * H, c, H, sum_post[c]);
-    if (GATE == kGateChannel) store8<float, true>(dst + static_cast<int64_t>(a.sum_gate) * H, c, H, sum_gate[c]);
+    store8<float, VEC>(dst, c, H, sum_pre[c]);
+    if (a.sum_post >= 0) store8<float, VEC>(dst + static_cast<int64_t>(a.sum_post) * H, c, H, sum_post[c]);
+    if (GATE == kGateChannel) store8<float, VEC>(dst + static_cast<int64_t>(a.sum_gate) * H, c, H, sum_gate[c]);
   }
 }
 
@@ -637,7 +686,14 @@ bool vector_rows(const NormArgs& a, int dtype) {
 }
 
 bool bad_common(const NormArgs& a, int dtype, int param_f32) {
-  return a.T < 0 || a.H < 1 || a.H > kMaxWidth || dtype < MOE_B200_F32 || dtype > MOE_B200_F16 || (param_f32 & ~7) ||
+  if (dtype < MOE_B200_F32 || dtype > MOE_B200_F16) return true;
+  const int size = element_size(dtype);
+  const void* const rows[] = {a.x, a.y, a.gh, a.gs, a.s, a.h, a.dx, a.dy};
+  for (const void* p : rows)
+    if (!aligned(p, size)) return true;
+  if (!aligned(a.pre_w, a.pre_f32 ? 4 : size) || !aligned(a.post_w, a.post_f32 ? 4 : size) || !aligned(a.gate, a.gate_f32 ? 4 : size))
+    return true;
+  return a.T < 0 || a.H < 1 || a.H > kMaxWidth || (param_f32 & ~7) ||
          a.gate_kind < kGateNone || a.gate_kind > kGateFull || (a.gate_kind != kGateNone && (!a.gate || !a.y)) ||
          (a.post_w && !a.y);
 }
@@ -654,21 +710,17 @@ int forward_arrays(const NormArgs& a, int size) {
 template <typename T, int CH, bool VEC, bool QUANT, int GATE>
 cudaError_t launch_forward(NormArgs a, int threads, cudaStream_t stream) {
   const auto kernel = block_norm_kernel<T, CH, VEC, QUANT, GATE>;
-  size_t smem = 0;
-  int per_sm = 8;
-  if (VEC) {
-    a.arrays = forward_arrays(a, sizeof(T));
-    const size_t stage = static_cast<size_t>(a.arrays) * CH * threads * sizeof(Pack8<T>);
-    // as many CTAs as the registers are cut for, or fewer where their rings do not fit; two stages at least, if
-    // that can be had
-    per_sm = 896 / threads > 0 ? 896 / threads : 1;
-    while (per_sm > 1 && 2 * stage * per_sm > kRingMost) per_sm /= 2;
-    a.ring = static_cast<int>(kRingMost / (stage * per_sm));
-    if (a.ring > kMaxRing) a.ring = kMaxRing;
-    smem = a.ring * stage;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
-  }
+  a.arrays = forward_arrays(a, sizeof(T));
+  const size_t stage = static_cast<size_t>(a.arrays) * (VEC ? CH * threads * sizeof(Pack8<T>) : span_bytes(a.H, sizeof(T)));
+  // as many CTAs as the registers are cut for, or fewer where their rings do not fit; two stages at least, if that can be
+  // had
+  int per_sm = 896 / threads > 0 ? 896 / threads : 1;
+  while (per_sm > 1 && 2 * stage * per_sm > kRingMost) per_sm /= 2;
+  a.ring = static_cast<int>(kRingMost / (stage * per_sm));
+  if (a.ring > kMaxRing) a.ring = kMaxRing;
+  const size_t smem = a.ring * stage;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
   return launch_pdl(kernel, dim3(grid_rows(a.T, per_sm)), dim3(threads), smem, stream, a);
 }
 
@@ -714,19 +766,19 @@ cudaError_t launch_backward(const NormArgs& a, int grid, int threads, cudaStream
   return launch_pdl(block_norm_backward_kernel<T, CH, VEC>, dim3(grid), dim3(threads), smem, stream, a);
 }
 
-template <typename T, int CH, int MAXT, int GATE>
+template <typename T, int CH, bool VEC, int GATE>
 cudaError_t launch_ring(const NormArgs& a, int grid, int threads, size_t smem, cudaStream_t stream) {
-  const auto kernel = block_norm_backward_ring_kernel<T, CH, MAXT, GATE>;
+  const auto kernel = block_norm_backward_ring_kernel<T, CH, VEC, GATE>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
   return launch_pdl(kernel, dim3(grid), dim3(threads), smem, stream, a);
 }
 
-template <typename T, int CH, int MAXT>
+template <typename T, int CH, bool VEC>
 cudaError_t launch_ring(const NormArgs& a, int grid, int threads, size_t smem, cudaStream_t stream) {
-  if (a.gate_kind == kGateChannel) return launch_ring<T, CH, MAXT, kGateChannel>(a, grid, threads, smem, stream);
-  if (a.gate_kind == kGateFull) return launch_ring<T, CH, MAXT, kGateFull>(a, grid, threads, smem, stream);
-  return launch_ring<T, CH, MAXT, kGateNone>(a, grid, threads, smem, stream);
+  if (a.gate_kind == kGateChannel) return launch_ring<T, CH, VEC, kGateChannel>(a, grid, threads, smem, stream);
+  if (a.gate_kind == kGateFull) return launch_ring<T, CH, VEC, kGateFull>(a, grid, threads, smem, stream);
+  return launch_ring<T, CH, VEC, kGateNone>(a, grid, threads, smem, stream);
 }
 
 template <typename T>
@@ -734,17 +786,18 @@ cudaError_t launch_backward(NormArgs a, const ColumnSumArgs& cs, bool vec, cudaS
   const Shape sh = shape_of(a.H);
   const int grid = cs.n_parts, nt = sh.threads;
   a.arrays = a.gate_kind == kGateFull ? 5 : 4;
-  const size_t array = static_cast<size_t>(sh.ch) * nt * sizeof(Pack8<T>), stage = a.arrays * array, weights = 3 * array;
+  const size_t array = static_cast<size_t>(sh.ch) * nt * sizeof(Pack8<T>), weights = 3 * array;
+  const size_t stage = a.arrays * (vec ? array : span_bytes(a.H, sizeof(T)));
   const bool own_type = sizeof(T) == 4 || !(a.pre_f32 || a.post_f32 || a.gate_f32);
   // the ring kernel wants two stages at least; a longer row or a mixed call takes the other one
   const size_t room = 220 * 1024 / (sh.ch == 1 ? 512 / nt : 1) - 2048;
   a.ring = room > weights ? static_cast<int>((room - weights) / stage) : 0;
   if (a.ring > kMaxRing) a.ring = kMaxRing;
   cudaError_t e;
-  if (vec && own_type && sh.ch <= 2 && a.ring >= 2) {
+  if (own_type && sh.ch <= 2 && a.ring >= 2) {
     const size_t smem = a.ring * stage + weights;
-    if (sh.ch == 1) e = launch_ring<T, 1, 256>(a, grid, nt, smem, stream);
-    else e = launch_ring<T, 2, 512>(a, grid, nt, smem, stream);
+    if (sh.ch == 1) e = vec ? launch_ring<T, 1, true>(a, grid, nt, smem, stream) : launch_ring<T, 1, false>(a, grid, nt, smem, stream);
+    else e = vec ? launch_ring<T, 2, true>(a, grid, nt, smem, stream) : launch_ring<T, 2, false>(a, grid, nt, smem, stream);
   } else if (sh.ch == 1) {
     e = vec ? launch_backward<T, 1, true>(a, grid, nt, stream) : launch_backward<T, 1, false>(a, grid, nt, stream);
   } else if (sh.ch == 2) {

@@ -100,6 +100,16 @@ NORM = [
     (4, 16384, F, "channel", True, True, 0, 0, False),
     (4, 16384, BF, "token", True, True, 0, 0, True),
     (3, 16383, BF, "full", True, True, 0, 0, False),
+    # rows that start anywhere, several per CTA, so that every stage of a ring is used again
+    (1900, 1001, BF, "channel", True, True, 0, 0, False),
+    (700, 4099, BF, "full", True, True, 0, 1, False),
+    (650, 3001, HF, "token", True, True, 5, 1, False),
+    (601, 5003, F, "channel", True, False, 2, 1, False),
+    (460, 8191, BF, "none", True, True, 0, 0, False),
+    (900, 2304, BF, "token", True, True, 3, 2, False),
+    (1500, 770, HF, "none", False, False, 0, 0, False),
+    (2500, 640, BF, "full", True, True, 0, 0, False),
+    (620, 7168, BF, "full", True, False, 8, 0, False),
 ]
 
 
