@@ -44,6 +44,12 @@ struct NormArgs {
   int n_sums, sum_post, sum_gate;            // rows of `partial`: 0 is dw_pre; -1: not wanted
 };
 
+// How rows are read and written.  kAligned: every row starts on 16 bytes.  kEdges: all row arrays are off by the same in
+// every row (an odd width, strides that differ from it by whole 16 bytes, aligned bases): blocks of 16 bytes are still
+// shared by loads and stores, the first and last one of a row are partial.  With a grid that is a multiple of eight, or
+// one row per CTA, a CTA's rows are all off by the same, so that its threads keep their columns.  kSpan: anything else.
+enum RowMode : int { kSpan = 0, kAligned = 1, kEdges = 2 };
+
 // Which column a thread's j-th element of chunk c is: eight neighbours where rows can be read 16 bytes at a time,
 // else columns blockDim.x apart, so that single-element loads of a warp are adjacent.
 template <bool VEC>
@@ -124,15 +130,64 @@ __device__ __forceinline__ uint32_t piece(int array, int c) {
   return (array * CH + c) * blockDim.x * sizeof(Pack8<T>) + threadIdx.x * 16;
 }
 
-template <typename T, int CH>
-__device__ __forceinline__ void fetch_row(uint32_t stage, int array, const T* row, int H) {
+// First column of a thread's group c where rows begin `off` elements behind 16 bytes.
+__device__ __forceinline__ int group_column(int c, int off) { return column<true>(c, 0) - off; }
+
+template <typename T, int CH, int MODE>
+__device__ __forceinline__ void fetch_row(uint32_t stage, int array, const T* row, int H, int off) {
+  constexpr int kBlockElems = 16 / static_cast<int>(sizeof(T));
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const int col = column<true>(c, 0);
+    const int col = group_column(c, off);
     if (col >= H) continue;
 #pragma unroll
-    for (int half = 0; half < static_cast<int>(sizeof(T)) / 2; ++half)
-      copy16(stage + piece<T, CH>(array, c) + half * 16 * blockDim.x, row + col + half * (16 / static_cast<int>(sizeof(T))), true);
+    for (int half = 0; half < static_cast<int>(sizeof(T)) / 2; ++half) {
+      const uint32_t to = stage + piece<T, CH>(array, c) + half * 16 * blockDim.x;
+      const int first = col + half * kBlockElems;
+      if (MODE == kAligned) copy16(to, row + first, true);
+      else if (first < H)    // the row's bytes and, in its first block, those in front of it
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(row + first),
+                     "r"(min(kBlockElems, H - first) * static_cast<int>(sizeof(T))) : "memory");
+    }
+  }
+}
+
+// Zeros where a group of eight columns from `col` lies outside the row.
+__device__ __forceinline__ void clip8(int col, int H, F2 (&v)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = get(v[j]);
+    v[j] = make_f2(col + 2 * j >= 0 && col + 2 * j < H ? f.x : 0.0f, col + 2 * j + 1 >= 0 && col + 2 * j + 1 < H ? f.y : 0.0f);
+  }
+}
+__device__ __forceinline__ bool partial(int col, int H) { return col < 0 || col + 8 > H; }
+
+// Eight columns from `col` on of a row that starts at p, outside it `fill`.
+template <typename T>
+__device__ __forceinline__ void load8_at(const T* p, int col, int H, float fill, F2 (&v)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int c0 = col + 2 * j, c1 = c0 + 1;
+    v[j] = make_f2(c0 >= 0 && c0 < H ? to_f32<T>(p[c0]) : fill, c1 >= 0 && c1 < H ? to_f32<T>(p[c1]) : fill);
+  }
+}
+
+template <typename T, int MODE>
+__device__ __forceinline__ void store_row8(T* p, int c, int H, int off, const F2 (&v)[4], bool whole_blocks = true) {
+  if (MODE != kEdges) {
+    store8<T, MODE == kAligned>(p, c, H, v);
+    return;
+  }
+  const int col = group_column(c, off);
+  if (whole_blocks && !partial(col, H)) {
+    *reinterpret_cast<Pack8<T>*>(p + col) = pack8<T>(v);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = get(v[j]);
+    if (col + 2 * j >= 0 && col + 2 * j < H) p[col + 2 * j] = from_f32<T>(f.x);
+    if (col + 2 * j + 1 >= 0 && col + 2 * j + 1 < H) p[col + 2 * j + 1] = from_f32<T>(f.y);
   }
 }
 
@@ -145,12 +200,20 @@ __device__ __forceinline__ void take8(const uint8_t* stage, int array, int c, F2
   unpack8<T>(raw, v);
 }
 
+template <typename T, int CH>
+__device__ __forceinline__ void put8(uint8_t* stage, int array, int c, const F2 (&v)[4]) {
+  const Pack8<T> raw = pack8<T>(v);
+#pragma unroll
+  for (int half = 0; half < static_cast<int>(sizeof(T)) / 2; ++half)
+    *reinterpret_cast<uint4*>(stage + piece<T, CH>(array, c) + half * 16 * blockDim.x) = raw.w[half];
+}
+
 // Pieces behind the row's end are never copied: they hold zeros.
 template <typename T, int CH>
-__device__ __forceinline__ void clear_ring_ends(uint8_t* ring, uint32_t stage_bytes, int stages, int arrays, int H) {
+__device__ __forceinline__ void clear_ring_ends(uint8_t* ring, uint32_t stage_bytes, int stages, int arrays, int H, int off) {
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    if (column<true>(c, 0) < H) continue;
+    if (!partial(group_column(c, off), H)) continue;
     for (int i = 0; i < stages * arrays; ++i)
       for (int half = 0; half < static_cast<int>(sizeof(T)) / 2; ++half)
         *reinterpret_cast<uint4*>(ring + i / arrays * stage_bytes + piece<T, CH>(i % arrays, c) + half * 16 * blockDim.x) = make_uint4(0u, 0u, 0u, 0u);
@@ -182,10 +245,11 @@ __device__ __forceinline__ void take_span8(const uint8_t* row, int c, int H, F2 
 // GATE: where the gate and the parameters' types are known (all of the activations' type), else kAnyGate.
 constexpr int kAnyGate = -1;
 
-template <typename T, int CH, bool VEC, bool QUANT, int GATE>
+template <typename T, int CH, int MODE, bool QUANT, int GATE>
 __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 3 : CH == 2 ? 2 : 1) block_norm_kernel(NormArgs a) {
   griddep_launch_dependents();
   griddep_wait();
+  constexpr bool VEC = MODE != kSpan;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float red[2][32];
   const int H = a.H;
@@ -194,9 +258,11 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 3 : CH
   // a full gate of another type than the activations' is read directly
   const bool full_in_ring = GATE == kGateFull || (GATE == kAnyGate && gate_kind == kGateFull && !(a.gate_f32 && sizeof(T) == 2));
   const int span = span_bytes(H, sizeof(T));
+  const int off = MODE == kEdges ? static_cast<int>(blockIdx.x * static_cast<int64_t>(H) % (16 / static_cast<int>(sizeof(T)))) : 0;
   const uint32_t stage_bytes = static_cast<uint32_t>(a.arrays * (VEC ? CH * blockDim.x * sizeof(Pack8<T>) : span));
   auto param = [&](const void* p, int f32, int64_t offset, int c, F2 (&v)[4]) {
-    if (GATE == kAnyGate) load8_param<T, VEC>(p, f32, offset, c, H, v);
+    if (MODE == kEdges) take8<T, CH>(ring + a.ring * stage_bytes, p == a.pre_w ? 0 : p == a.post_w ? 1 : 2, c, v);
+    else if (GATE == kAnyGate) load8_param<T, VEC>(p, f32, offset, c, H, v);
     else load8<T, VEC>(static_cast<const T*>(p) + offset, c, H, v);
   };
   // rows still to be fetched and to be stored
@@ -208,9 +274,9 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 3 : CH
   auto fetch = [&](uint32_t stage) {
     if (fetch_at < a.T) {
       if (VEC) {
-        fetch_row<T, CH>(stage, 0, fetch_x, H);
-        if (a.y) fetch_row<T, CH>(stage, 1, fetch_y, H);
-        if (full_in_ring) fetch_row<T, CH>(stage, 2, fetch_g, H);
+        fetch_row<T, CH, MODE>(stage, 0, fetch_x, H, off);
+        if (a.y) fetch_row<T, CH, MODE>(stage, 1, fetch_y, H, off);
+        if (full_in_ring) fetch_row<T, CH, MODE>(stage, 2, fetch_g, H, off);
       } else {
         fetch_span(stage, fetch_x, H);
         if (a.y) fetch_span(stage + span, fetch_y, H);
@@ -228,8 +294,22 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 3 : CH
   auto take = [&](const uint8_t* stage, int array, const T* from, int c, F2 (&v)[4]) {
     if (VEC) take8<T, CH>(stage, array, c, v);
     else take_span8<T>(stage + array * span + row_low(from), c, H, v);
+    if (MODE == kEdges && partial(group_column(c, off), H)) clip8(group_column(c, off), H, v);
   };
-  if (VEC) clear_ring_ends<T, CH>(ring, stage_bytes, a.ring, a.arrays, H);
+  if (MODE == kEdges) {                            // the parameters at the thread's columns, behind the ring
+    const void* const from[3] = {a.pre_w, a.post_w, gate_kind == kGateChannel ? a.gate : nullptr};
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      if (!from[k]) continue;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        F2 w[4];
+        load8_at<T>(static_cast<const T*>(from[k]), group_column(c, off), H, 0.0f, w);
+        put8<T, CH>(ring + a.ring * stage_bytes, k, c, w);
+      }
+    }
+  }
+  if (VEC) clear_ring_ends<T, CH>(ring, stage_bytes, a.ring, a.arrays, H, off);
   for (int i = 0; i < a.ring; ++i) fetch(smem_address(ring) + i * stage_bytes);
   T* s_out = static_cast<T*>(a.s) + blockIdx.x * static_cast<int64_t>(H);
   T* h_out = static_cast<T*>(a.h) + blockIdx.x * static_cast<int64_t>(H);
@@ -284,7 +364,7 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 3 : CH
       for (int c = 0; c < CH; ++c) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[c][j] = fma2(aa, s[c][j], mul2(kk, n[c][j]));
-        store8<T, VEC>(s_out, c, H, s[c]);
+        store_row8<T, MODE>(s_out, c, H, off, s[c]);
       }
     }
     if (VEC) fetch(smem_address(stage));
@@ -331,7 +411,7 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 3 : CH
           if ((threadIdx.x & 15) == 0) a.q_scale[static_cast<int64_t>(col / kBlock) * a.T + row] = amax * (1.0f / 448.0f);
         }
       } else {
-        store8<T, VEC>(h_out, c, H, s[c]);
+        store_row8<T, MODE>(h_out, c, H, off, s[c]);
       }
     }
     s_out += step_h;
@@ -470,18 +550,20 @@ __global__ void __launch_bounds__(kNormThreads) block_norm_backward_kernel(NormA
 // rows come through a ring like the forward's, the column sums stay in registers as fp32, and the weights, which leave no
 // registers for themselves, in shared memory behind the ring (an SM's quarter has 128 registers for each of four warps).
 // Missing parts are neutral values (y = 0, w_post = 1, gate = 1) instead of branches.
-template <typename T, int CH, bool VEC, int GATE>
+template <typename T, int CH, int MODE, int GATE>
 __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 2 : 1) block_norm_backward_ring_kernel(NormArgs a) {
   griddep_launch_dependents();
   griddep_wait();
+  constexpr bool VEC = MODE != kSpan;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float red[2][96];
   const int H = a.H;
   const float inv_h = 1.0f / static_cast<float>(H), scale = a.y ? a.a : 1.0f;
   const int span = span_bytes(H, sizeof(T));
+  const int off = MODE == kEdges ? static_cast<int>(blockIdx.x * static_cast<int64_t>(H) % (16 / static_cast<int>(sizeof(T)))) : 0;
   const uint32_t stage_bytes = static_cast<uint32_t>(a.arrays * (VEC ? CH * blockDim.x * sizeof(Pack8<T>) : span));
   auto fetch_one = [&](uint32_t stage, int array, const void* p, int64_t at) {
-    if (VEC) fetch_row<T, CH>(stage, array, static_cast<const T*>(p) + at, H);
+    if (VEC) fetch_row<T, CH, MODE>(stage, array, static_cast<const T*>(p) + at, H, off);
     else fetch_span(stage + array * span, static_cast<const T*>(p) + at, H);
   };
   // arrays of a stage: x, grad_h, grad_stream, y, gate; what the call lacks is never copied and stays zero
@@ -503,6 +585,7 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 2 : 1)
     if (VEC) take8<T, CH>(stage, array, c, v);
     else if (p) take_span8<T>(stage + array * span + row_low(static_cast<const T*>(p) + at), c, H, v);
     else v[0] = v[1] = v[2] = v[3] = both(0.0f);
+    if (MODE == kEdges && partial(group_column(c, off), H)) clip8(group_column(c, off), H, v);
   };
   uint8_t* const weights = ring + a.ring * stage_bytes;    // w_pre, w_post, gate per channel: the thread's own pieces
   F2 sum_pre[CH][4], sum_post[CH][4], sum_gate[GATE == kGateChannel ? CH : 1][4];
@@ -512,11 +595,11 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 2 : 1)
 #pragma unroll
     for (int k = 0; k < (GATE == kGateChannel ? 3 : 2); ++k) {
       F2 w[4] = {both(1.0f), both(1.0f), both(1.0f), both(1.0f)};
-      if (from[k]) load8<T, VEC>(static_cast<const T*>(from[k]), c, H, w);
-      const Pack8<T> v = pack8<T>(w);
-#pragma unroll
-      for (int half = 0; half < static_cast<int>(sizeof(T)) / 2; ++half)
-        *reinterpret_cast<uint4*>(weights + piece<T, CH>(k, c) + half * 16 * blockDim.x) = v.w[half];
+      if (from[k]) {
+        if (MODE == kEdges) load8_at<T>(static_cast<const T*>(from[k]), group_column(c, off), H, 1.0f, w);
+        else load8<T, VEC>(static_cast<const T*>(from[k]), c, H, w);
+      }
+      put8<T, CH>(weights, k, c, w);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -590,7 +673,7 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 2 : 1)
         d[c][j] = fma2(both(-k2), sh[c][j], d[c][j]);
         out[j] = mul2(both(scale), d[c][j]);
       }
-      store8<T, VEC>(static_cast<T*>(a.dx) + static_cast<int64_t>(row) * H, c, H, out);
+      store_row8<T, MODE>(static_cast<T*>(a.dx) + static_cast<int64_t>(row) * H, c, H, off, out);
       if (!a.y) continue;
       take(stage, 3, a.y, row * a.y_stride, c, yh);               // read again: registers are what this kernel is short of
       take8<T, CH>(weights, 1, c, wp);
@@ -605,7 +688,7 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 2 : 1)
           if (GATE == kGateChannel) sum_gate[c][j] = fma2(d[c][j], n, sum_gate[c][j]);
           else out[j] = mul2(d[c][j], n);
         }
-        if (GATE == kGateFull) store8<T, VEC>(static_cast<T*>(a.dgate_rows) + static_cast<int64_t>(row) * H, c, H, out);
+        if (GATE == kGateFull) store_row8<T, MODE>(static_cast<T*>(a.dgate_rows) + static_cast<int64_t>(row) * H, c, H, off, out);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -613,7 +696,7 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 2 : 1)
         sum_post[c][j] = fma2(dn, yh[j], sum_post[c][j]);
         out[j] = fma2(both(-k1), yh[j], mul2(mul2(dn, wp[j]), both(r1)));
       }
-      store8<T, VEC>(static_cast<T*>(a.dy) + static_cast<int64_t>(row) * H, c, H, out);
+      store_row8<T, MODE>(static_cast<T*>(a.dy) + static_cast<int64_t>(row) * H, c, H, off, out);
     }
     if (VEC) fetch(row + static_cast<int64_t>(a.ring) * gridDim.x, smem_address(stage));
     slot = slot + 1 == a.ring ? 0 : slot + 1;
@@ -621,9 +704,9 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 2 : 1)
   float* dst = a.partial + static_cast<int64_t>(blockIdx.x) * a.n_sums * H;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    store8<float, VEC>(dst, c, H, sum_pre[c]);
-    if (a.sum_post >= 0) store8<float, VEC>(dst + static_cast<int64_t>(a.sum_post) * H, c, H, sum_post[c]);
-    if (GATE == kGateChannel) store8<float, VEC>(dst + static_cast<int64_t>(a.sum_gate) * H, c, H, sum_gate[c]);
+    store_row8<float, MODE>(dst, c, H, off, sum_pre[c], false);
+    if (a.sum_post >= 0) store_row8<float, MODE>(dst + static_cast<int64_t>(a.sum_post) * H, c, H, off, sum_post[c], false);
+    if (GATE == kGateChannel) store_row8<float, MODE>(dst + static_cast<int64_t>(a.sum_gate) * H, c, H, off, sum_gate[c], false);
   }
 }
 
@@ -670,20 +753,31 @@ Shape shape_of(int H) {
   return {ch, ((groups + ch - 1) / ch + 31) / 32 * 32};
 }
 
-// Rows can be moved 16 bytes at a time.
-bool rows_aligned(const void* p, int64_t stride, int size) {
-  return !p || (aligned(p, 16) && stride * size % 16 == 0);
+// How the rows of this call can be moved; for kEdges parameters need the activations' type too.
+RowMode row_mode(const NormArgs& a, int dtype) {
+  const int size = element_size(dtype), block = 16 / size;
+  struct { const void* p; int64_t stride; int size; } const rows[] = {
+      {a.x, a.x_stride, size}, {a.y, a.y_stride, size}, {a.gh, a.gh_stride, size}, {a.gs, a.gs_stride, size},
+      {a.s, a.H, size}, {a.h, a.H, size}, {a.dx, a.H, size}, {a.dy, a.H, size},
+      {a.gate_kind == kGateFull ? a.gate : nullptr, a.gate_stride, a.gate_f32 ? 4 : size},
+      {a.gate_kind == kGateFull ? a.dgate_rows : nullptr, a.H, a.gate_f32 ? 4 : size}};
+  bool all = a.H % 8 == 0, congruent = true;
+  for (const auto& r : rows) {
+    if (!r.p || aligned(r.p, 16)) {
+      all = all && (!r.p || r.stride * r.size % 16 == 0);
+      congruent = congruent && (!r.p || ((r.stride - a.H) % block == 0 && r.size == size));
+    } else {
+      all = congruent = false;
+    }
+  }
+  const bool params = aligned(a.pre_w, 16) && aligned(a.post_w, 16) && (a.gate_kind != kGateChannel || aligned(a.gate, 16));
+  if (all && params && aligned(a.q, 8)) return kAligned;
+  const bool own_type = size == 4 || !(a.pre_f32 || a.post_f32 || a.gate_f32);
+  return congruent && own_type && !a.q && shape_of(a.H + 7).ch <= 2 ? kEdges : kSpan;
 }
 
-bool vector_rows(const NormArgs& a, int dtype) {
-  const int size = element_size(dtype);
-  return a.H % 8 == 0 && rows_aligned(a.x, a.x_stride, size) && rows_aligned(a.y, a.y_stride, size) &&
-         (a.gate_kind == kGateToken || rows_aligned(a.gate, a.gate_kind == kGateFull ? a.gate_stride : 0, a.gate_f32 ? 4 : size)) &&
-         rows_aligned(a.pre_w, 0, 1) && rows_aligned(a.post_w, 0, 1) && rows_aligned(a.gh, a.gh_stride, size) &&
-         rows_aligned(a.gs, a.gs_stride, size) && rows_aligned(a.s, a.H, size) && rows_aligned(a.h, a.H, size) &&
-         rows_aligned(a.dx, a.H, size) && rows_aligned(a.dy, a.H, size) &&
-         (a.gate_kind != kGateFull || rows_aligned(a.dgate_rows, a.H, a.gate_f32 ? 4 : size)) && aligned(a.q, 8);
-}
+// Width by which threads are counted: with kEdges a row has up to one block more.
+int counted_width(int H, RowMode mode) { return mode == kEdges ? H + 7 : H; }
 
 bool bad_common(const NormArgs& a, int dtype, int param_f32) {
   if (dtype < MOE_B200_F32 || dtype > MOE_B200_F16) return true;
@@ -700,61 +794,65 @@ bool bad_common(const NormArgs& a, int dtype, int param_f32) {
 
 constexpr size_t kRingMost = 208 * 1024;          // shared memory of an SM for rings; the rest is first-level cache
 
-int grid_rows(int T, int per_sm) { return T < kNumSMs * per_sm ? T : kNumSMs * per_sm; }
+int grid_rows(int T, int per_sm, RowMode mode) {
+  if (T <= kNumSMs * per_sm) return T;
+  return mode == kEdges ? kNumSMs * per_sm / 8 * 8 : kNumSMs * per_sm;
+}
 
 // Activations that a row's ring stage holds: x, y and a full gate of the same type.
 int forward_arrays(const NormArgs& a, int size) {
   return 1 + (a.y ? 1 : 0) + (a.gate_kind == kGateFull && (!a.gate_f32 || size == 4) ? 1 : 0);
 }
 
-template <typename T, int CH, bool VEC, bool QUANT, int GATE>
+template <typename T, int CH, RowMode MODE, bool QUANT, int GATE>
 cudaError_t launch_forward(NormArgs a, int threads, cudaStream_t stream) {
-  const auto kernel = block_norm_kernel<T, CH, VEC, QUANT, GATE>;
+  const auto kernel = block_norm_kernel<T, CH, MODE, QUANT, GATE>;
   a.arrays = forward_arrays(a, sizeof(T));
-  const size_t stage = static_cast<size_t>(a.arrays) * (VEC ? CH * threads * sizeof(Pack8<T>) : span_bytes(a.H, sizeof(T)));
+  const size_t stage = static_cast<size_t>(a.arrays) * (MODE != kSpan ? CH * threads * sizeof(Pack8<T>) : span_bytes(a.H, sizeof(T)));
+  const size_t weights = MODE == kEdges ? 3 * CH * threads * sizeof(Pack8<T>) : 0;
   // as many CTAs as the registers are cut for, or fewer where their rings do not fit; two stages at least, if that can be
   // had
   int per_sm = 896 / threads > 0 ? 896 / threads : 1;
-  while (per_sm > 1 && 2 * stage * per_sm > kRingMost) per_sm /= 2;
-  a.ring = static_cast<int>(kRingMost / (stage * per_sm));
+  while (per_sm > 1 && (2 * stage + weights) * per_sm > kRingMost) per_sm /= 2;
+  a.ring = static_cast<int>((kRingMost / per_sm - weights) / stage);
   if (a.ring > kMaxRing) a.ring = kMaxRing;
-  const size_t smem = a.ring * stage;
+  const size_t smem = a.ring * stage + weights;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
-  return launch_pdl(kernel, dim3(grid_rows(a.T, per_sm)), dim3(threads), smem, stream, a);
+  return launch_pdl(kernel, dim3(grid_rows(a.T, per_sm, MODE)), dim3(threads), smem, stream, a);
 }
 
-template <typename T, int CH, bool QUANT>
+template <typename T, int CH, RowMode MODE, bool QUANT>
 cudaError_t launch_forward(const NormArgs& a, int threads, cudaStream_t stream) {
-  const bool own_type = sizeof(T) == 4 || !(a.pre_f32 || a.post_f32 || a.gate_f32);
-  if (own_type && CH <= 2) {
-    constexpr int kCh = CH <= 2 ? CH : 1;
-    if (a.gate_kind == kGateChannel) return launch_forward<T, kCh, true, QUANT, kGateChannel>(a, threads, stream);
-    if (a.gate_kind == kGateFull) return launch_forward<T, kCh, true, QUANT, kGateFull>(a, threads, stream);
-    return launch_forward<T, kCh, true, QUANT, kGateNone>(a, threads, stream);
-  }
-  return launch_forward<T, CH, true, QUANT, kAnyGate>(a, threads, stream);
+  if (a.gate_kind == kGateChannel) return launch_forward<T, CH, MODE, QUANT, kGateChannel>(a, threads, stream);
+  if (a.gate_kind == kGateFull) return launch_forward<T, CH, MODE, QUANT, kGateFull>(a, threads, stream);
+  return launch_forward<T, CH, MODE, QUANT, kGateNone>(a, threads, stream);
 }
 
+// `known`: the gate is compiled in (parameters have the activations' type and a thread has at most 16 columns).
 template <typename T, int CH>
-cudaError_t launch_forward(const NormArgs& a, bool vec, int threads, cudaStream_t stream) {
-  if (a.q) return launch_forward<T, CH, true>(a, threads, stream);
-  if (vec) return launch_forward<T, CH, false>(a, threads, stream);
-  return launch_forward<T, CH, false, false, kAnyGate>(a, threads, stream);
+cudaError_t launch_forward(const NormArgs& a, RowMode mode, bool known, int threads, cudaStream_t stream) {
+  constexpr int kCh = CH <= 2 ? CH : 1;
+  if (mode == kEdges) return launch_forward<T, kCh, kEdges, false>(a, threads, stream);
+  if (mode == kSpan) return launch_forward<T, CH, kSpan, false, kAnyGate>(a, threads, stream);
+  if (known) return a.q ? launch_forward<T, kCh, kAligned, true>(a, threads, stream) : launch_forward<T, kCh, kAligned, false>(a, threads, stream);
+  return a.q ? launch_forward<T, CH, kAligned, true, kAnyGate>(a, threads, stream)
+             : launch_forward<T, CH, kAligned, false, kAnyGate>(a, threads, stream);
 }
 
 template <typename T>
-cudaError_t launch_forward(const NormArgs& a, bool vec, cudaStream_t stream) {
-  const Shape sh = shape_of(a.H);
-  if (sh.ch == 1) return launch_forward<T, 1>(a, vec, sh.threads, stream);
-  if (sh.ch == 2) return launch_forward<T, 2>(a, vec, sh.threads, stream);
-  return launch_forward<T, 4>(a, vec, sh.threads, stream);
+cudaError_t launch_forward(const NormArgs& a, RowMode mode, cudaStream_t stream) {
+  const Shape sh = shape_of(counted_width(a.H, mode));
+  const bool known = sh.ch <= 2 && (sizeof(T) == 4 || !(a.pre_f32 || a.post_f32 || a.gate_f32));
+  if (sh.ch == 1) return launch_forward<T, 1>(a, mode, known, sh.threads, stream);
+  if (sh.ch == 2) return launch_forward<T, 2>(a, mode, known, sh.threads, stream);
+  return launch_forward<T, 4>(a, mode, known, sh.threads, stream);
 }
 
 // CTAs of the backward pass, one partial row of column sums each: as many as the registers hold.
-int backward_parts(int T, int H) {
-  const Shape sh = shape_of(H);
-  return grid_rows(T, sh.ch > 1 ? 1 : 512 / sh.threads);
+int backward_parts(int T, int H, RowMode mode) {
+  const Shape sh = shape_of(counted_width(H, mode));
+  return grid_rows(T, sh.ch > 1 ? 1 : 512 / sh.threads, mode);
 }
 
 template <typename T, int CH, bool VEC>
@@ -766,38 +864,59 @@ cudaError_t launch_backward(const NormArgs& a, int grid, int threads, cudaStream
   return launch_pdl(block_norm_backward_kernel<T, CH, VEC>, dim3(grid), dim3(threads), smem, stream, a);
 }
 
-template <typename T, int CH, bool VEC, int GATE>
+// Whether the ring kernel takes this call (a longer row or a mixed call goes to the other one), its stages and memory.
+template <typename T>
+bool ring_plan(NormArgs& a, RowMode mode, size_t* smem) {
+  const Shape sh = shape_of(counted_width(a.H, mode));
+  if (sh.ch > 2 || (sizeof(T) == 2 && (a.pre_f32 || a.post_f32 || a.gate_f32))) return false;
+  a.arrays = a.gate_kind == kGateFull ? 5 : 4;
+  const size_t array = static_cast<size_t>(sh.ch) * sh.threads * sizeof(Pack8<T>), weights = 3 * array;
+  const size_t stage = a.arrays * (mode != kSpan ? array : span_bytes(a.H, sizeof(T)));
+  const size_t room = 220 * 1024 / (sh.ch == 1 ? 512 / sh.threads : 1) - 2048;
+  a.ring = room > weights ? static_cast<int>((room - weights) / stage) : 0;
+  if (a.ring > kMaxRing) a.ring = kMaxRing;
+  *smem = a.ring * stage + weights;
+  return a.ring >= 2;
+}
+template <typename T>
+bool ring_fits(NormArgs a, RowMode mode) {
+  size_t smem;
+  return ring_plan<T>(a, mode, &smem);
+}
+
+template <typename T, int CH, RowMode MODE, int GATE>
 cudaError_t launch_ring(const NormArgs& a, int grid, int threads, size_t smem, cudaStream_t stream) {
-  const auto kernel = block_norm_backward_ring_kernel<T, CH, VEC, GATE>;
+  const auto kernel = block_norm_backward_ring_kernel<T, CH, MODE, GATE>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
   return launch_pdl(kernel, dim3(grid), dim3(threads), smem, stream, a);
 }
 
-template <typename T, int CH, bool VEC>
+template <typename T, int CH, RowMode MODE>
 cudaError_t launch_ring(const NormArgs& a, int grid, int threads, size_t smem, cudaStream_t stream) {
-  if (a.gate_kind == kGateChannel) return launch_ring<T, CH, VEC, kGateChannel>(a, grid, threads, smem, stream);
-  if (a.gate_kind == kGateFull) return launch_ring<T, CH, VEC, kGateFull>(a, grid, threads, smem, stream);
-  return launch_ring<T, CH, VEC, kGateNone>(a, grid, threads, smem, stream);
+  if (a.gate_kind == kGateChannel) return launch_ring<T, CH, MODE, kGateChannel>(a, grid, threads, smem, stream);
+  if (a.gate_kind == kGateFull) return launch_ring<T, CH, MODE, kGateFull>(a, grid, threads, smem, stream);
+  return launch_ring<T, CH, MODE, kGateNone>(a, grid, threads, smem, stream);
+}
+
+template <typename T, int CH>
+cudaError_t launch_ring(const NormArgs& a, RowMode mode, int grid, int threads, size_t smem, cudaStream_t stream) {
+  if (mode == kAligned) return launch_ring<T, CH, kAligned>(a, grid, threads, smem, stream);
+  if (mode == kEdges) return launch_ring<T, CH, kEdges>(a, grid, threads, smem, stream);
+  return launch_ring<T, CH, kSpan>(a, grid, threads, smem, stream);
 }
 
 template <typename T>
-cudaError_t launch_backward(NormArgs a, const ColumnSumArgs& cs, bool vec, cudaStream_t stream) {
-  const Shape sh = shape_of(a.H);
+cudaError_t launch_backward(NormArgs a, ColumnSumArgs cs, RowMode mode, cudaStream_t stream) {
+  if (mode == kEdges && !ring_fits<T>(a, mode)) mode = kSpan;
+  const Shape sh = shape_of(counted_width(a.H, mode));
+  cs.n_parts = backward_parts(a.T, a.H, mode);
   const int grid = cs.n_parts, nt = sh.threads;
-  a.arrays = a.gate_kind == kGateFull ? 5 : 4;
-  const size_t array = static_cast<size_t>(sh.ch) * nt * sizeof(Pack8<T>), weights = 3 * array;
-  const size_t stage = a.arrays * (vec ? array : span_bytes(a.H, sizeof(T)));
-  const bool own_type = sizeof(T) == 4 || !(a.pre_f32 || a.post_f32 || a.gate_f32);
-  // the ring kernel wants two stages at least; a longer row or a mixed call takes the other one
-  const size_t room = 220 * 1024 / (sh.ch == 1 ? 512 / nt : 1) - 2048;
-  a.ring = room > weights ? static_cast<int>((room - weights) / stage) : 0;
-  if (a.ring > kMaxRing) a.ring = kMaxRing;
+  size_t smem = 0;
+  const bool vec = mode == kAligned;
   cudaError_t e;
-  if (own_type && sh.ch <= 2 && a.ring >= 2) {
-    const size_t smem = a.ring * stage + weights;
-    if (sh.ch == 1) e = vec ? launch_ring<T, 1, true>(a, grid, nt, smem, stream) : launch_ring<T, 1, false>(a, grid, nt, smem, stream);
-    else e = vec ? launch_ring<T, 2, true>(a, grid, nt, smem, stream) : launch_ring<T, 2, false>(a, grid, nt, smem, stream);
+  if (ring_plan<T>(a, mode, &smem)) {
+    e = sh.ch == 1 ? launch_ring<T, 1>(a, mode, grid, nt, smem, stream) : launch_ring<T, 2>(a, mode, grid, nt, smem, stream);
   } else if (sh.ch == 1) {
     e = vec ? launch_backward<T, 1, true>(a, grid, nt, stream) : launch_backward<T, 1, false>(a, grid, nt, stream);
   } else if (sh.ch == 2) {
@@ -835,19 +954,24 @@ extern "C" int moe_fp8_block_scale_block_norm(const void* x, int64_t x_stride, c
   if (bad_common(a, dtype, param_f32) || !(eps > 0.0f)) return MOE_B200_EINVAL;
   if (T == 0) return MOE_B200_OK;
   if (!x || !pre_weight || !h || !rstd || !aligned(rstd, 8) || (y && !stream_out)) return MOE_B200_EINVAL;
-  const bool vec = vector_rows(a, dtype);
-  if (h_scale && (H % kBlock != 0 || !vec)) return MOE_B200_EINVAL;
+  const RowMode mode = row_mode(a, dtype);
+  if (h_scale && (H % kBlock != 0 || mode != kAligned)) return MOE_B200_EINVAL;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   cudaError_t e;
-  if (dtype == MOE_B200_F32) e = launch_forward<float>(a, vec, stream);
-  else if (dtype == MOE_B200_BF16) e = launch_forward<__nv_bfloat16>(a, vec, stream);
-  else e = launch_forward<__half>(a, vec, stream);
+  if (dtype == MOE_B200_F32) e = launch_forward<float>(a, mode, stream);
+  else if (dtype == MOE_B200_BF16) e = launch_forward<__nv_bfloat16>(a, mode, stream);
+  else e = launch_forward<__half>(a, mode, stream);
   return launch_status(e, 1);
 }
 
 extern "C" size_t moe_fp8_block_scale_block_norm_backward_workspace_bytes(int T, int H) {
   if (T < 0 || H < 1 || H > kMaxWidth) return 0;
-  return static_cast<size_t>(backward_parts(T, H)) * 3 * H * sizeof(float);
+  int parts = 0;
+  for (RowMode mode : {kSpan, kAligned, kEdges}) {
+    const int n = backward_parts(T, H, mode);
+    parts = n > parts ? n : parts;
+  }
+  return static_cast<size_t>(parts) * 3 * H * sizeof(float);
 }
 
 extern "C" int moe_fp8_block_scale_block_norm_backward(
@@ -889,14 +1013,13 @@ extern "C" int moe_fp8_block_scale_block_norm_backward(
   }
   a.partial = static_cast<float*>(workspace);
   cs.partial = a.partial;
-  cs.n_parts = backward_parts(T, H);
   cs.n_sums = a.n_sums;
   cs.H = H;
-  const bool vec = vector_rows(a, dtype);
+  const RowMode mode = row_mode(a, dtype);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   cudaError_t e;
-  if (dtype == MOE_B200_F32) e = launch_backward<float>(a, cs, vec, stream);
-  else if (dtype == MOE_B200_BF16) e = launch_backward<__nv_bfloat16>(a, cs, vec, stream);
-  else e = launch_backward<__half>(a, cs, vec, stream);
+  if (dtype == MOE_B200_F32) e = launch_backward<float>(a, cs, mode, stream);
+  else if (dtype == MOE_B200_BF16) e = launch_backward<__nv_bfloat16>(a, cs, mode, stream);
+  else e = launch_backward<__half>(a, cs, mode, stream);
   return launch_status(e, 2);
 }
