@@ -398,8 +398,8 @@ cudaError_t launch_chunks(const BalanceArgs& a, bool backward, cudaStream_t stre
   }
   constexpr int kChunkWarps = chunk_warps(EPL);
   const size_t smem = static_cast<size_t>(kChunkWarps + 1) * a.E * 4;
-  const cudaError_t e = cudaFuncSetAttribute(balance_chunk_kernel<T, EPL, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (kChunkWarps + 1) * EPL * 32 * 4);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(balance_chunk_kernel<T, EPL, VEC>, (kChunkWarps + 1) * EPL * 32 * 4, done);
   if (e != cudaSuccess) return e;
   return launch_pdl(balance_chunk_kernel<T, EPL, VEC>, dim3(a.n_chunks), dim3(32 * kChunkWarps), smem, stream, a);
 }

@@ -47,8 +47,12 @@ struct NormArgs {
 // How rows are read and written.  kAligned: every row starts on 16 bytes.  kEdges: all row arrays are off by the same in
 // every row (an odd width, strides that differ from it by whole 16 bytes, aligned bases): blocks of 16 bytes are still
 // shared by loads and stores, the first and last one of a row are partial.  With a grid that is a multiple of eight, or
-// one row per CTA, a CTA's rows are all off by the same, so that its threads keep their columns.  kSpan: anything else.
-enum RowMode : int { kSpan = 0, kAligned = 1, kEdges = 2 };
+// one row per CTA, a CTA's rows are all off by the same, so that its threads keep their columns.  kShifted: the results are
+// such rows, the inputs start anywhere: they come as the aligned blocks that cover them and are shifted when they are read.
+// kSpan: anything else, element by element.
+enum RowMode : int { kSpan = 0, kAligned = 1, kEdges = 2, kShifted = 3 };
+__host__ __device__ constexpr bool by_block(RowMode m) { return m == kAligned || m == kEdges; }     // a thread reads what it copied
+__host__ __device__ constexpr bool has_edges(RowMode m) { return m == kEdges || m == kShifted; }    // columns begin in front of the row
 
 // Which column a thread's j-th element of chunk c is: eight neighbours where rows can be read 16 bytes at a time,
 // else columns blockDim.x apart, so that single-element loads of a warp are adjacent.
@@ -133,7 +137,7 @@ __device__ __forceinline__ uint32_t piece(int array, int c) {
 // First column of a thread's group c where rows begin `off` elements behind 16 bytes.
 __device__ __forceinline__ int group_column(int c, int off) { return column<true>(c, 0) - off; }
 
-template <typename T, int CH, int MODE>
+template <typename T, int CH, RowMode MODE>
 __device__ __forceinline__ void fetch_row(uint32_t stage, int array, const T* row, int H, int off) {
   constexpr int kBlockElems = 16 / static_cast<int>(sizeof(T));
 #pragma unroll
@@ -172,9 +176,9 @@ __device__ __forceinline__ void load8_at(const T* p, int col, int H, float fill,
   }
 }
 
-template <typename T, int MODE>
+template <typename T, RowMode MODE>
 __device__ __forceinline__ void store_row8(T* p, int c, int H, int off, const F2 (&v)[4], bool whole_blocks = true) {
-  if (MODE != kEdges) {
+  if (!has_edges(MODE)) {
     store8<T, MODE == kAligned>(p, c, H, v);
     return;
   }
@@ -237,6 +241,27 @@ __device__ __forceinline__ void fetch_span(uint32_t to, const T* row, int H) {
 template <typename T>
 __device__ __forceinline__ int row_low(const T* row) { return static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15); }
 
+// Eight columns from `col` on of a row in shared memory that starts at `row`, on any element.
+__device__ __forceinline__ void shifted8(const uint8_t* at, F2 (&v)[4], float) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = make_f2(reinterpret_cast<const float*>(at)[2 * j], reinterpret_cast<const float*>(at)[2 * j + 1]);
+}
+template <typename T>
+__device__ __forceinline__ void shifted8(const uint8_t* at, F2 (&v)[4], T) {
+  const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(at) & 2) * 8;
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(at - odd / 8);
+  uint32_t w[5];
+#pragma unroll
+  for (int j = 0; j < 5; ++j) w[j] = words[j];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = unpack2(__funnelshift_r(w[j], w[j + 1], odd), T());
+}
+template <typename T>
+__device__ __forceinline__ void take_shifted8(const uint8_t* row, int col, int H, F2 (&v)[4]) {
+  if (partial(col, H)) load8_at<T>(reinterpret_cast<const T*>(row), col, H, 0.0f, v);
+  else shifted8(row + col * static_cast<int>(sizeof(T)), v, T());
+}
+
 template <typename T>
 __device__ __forceinline__ void take_span8(const uint8_t* row, int c, int H, F2 (&v)[4]) {
   load8<T, false>(reinterpret_cast<const T*>(row), c, H, v);
@@ -245,11 +270,11 @@ __device__ __forceinline__ void take_span8(const uint8_t* row, int c, int H, F2 
 // GATE: where the gate and the parameters' types are known (all of the activations' type), else kAnyGate.
 constexpr int kAnyGate = -1;
 
-template <typename T, int CH, int MODE, bool QUANT, int GATE>
+template <typename T, int CH, RowMode MODE, bool QUANT, int GATE>
 __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 3 : CH == 2 ? 2 : 1) block_norm_kernel(NormArgs a) {
   griddep_launch_dependents();
   griddep_wait();
-  constexpr bool VEC = MODE != kSpan;
+  constexpr bool VEC = by_block(MODE);
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float red[2][32];
   const int H = a.H;
@@ -258,10 +283,10 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 3 : CH
   // a full gate of another type than the activations' is read directly
   const bool full_in_ring = GATE == kGateFull || (GATE == kAnyGate && gate_kind == kGateFull && !(a.gate_f32 && sizeof(T) == 2));
   const int span = span_bytes(H, sizeof(T));
-  const int off = MODE == kEdges ? static_cast<int>(blockIdx.x * static_cast<int64_t>(H) % (16 / static_cast<int>(sizeof(T)))) : 0;
+  const int off = has_edges(MODE) ? static_cast<int>(blockIdx.x * static_cast<int64_t>(H) % (16 / static_cast<int>(sizeof(T)))) : 0;
   const uint32_t stage_bytes = static_cast<uint32_t>(a.arrays * (VEC ? CH * blockDim.x * sizeof(Pack8<T>) : span));
   auto param = [&](const void* p, int f32, int64_t offset, int c, F2 (&v)[4]) {
-    if (MODE == kEdges) take8<T, CH>(ring + a.ring * stage_bytes, p == a.pre_w ? 0 : p == a.post_w ? 1 : 2, c, v);
+    if (has_edges(MODE)) take8<T, CH>(ring + a.ring * stage_bytes, p == a.pre_w ? 0 : p == a.post_w ? 1 : 2, c, v);
     else if (GATE == kAnyGate) load8_param<T, VEC>(p, f32, offset, c, H, v);
     else load8<T, VEC>(static_cast<const T*>(p) + offset, c, H, v);
   };
@@ -293,10 +318,11 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 3 : CH
   const T *row_x = fetch_x, *row_y = fetch_y, *row_g = fetch_g;
   auto take = [&](const uint8_t* stage, int array, const T* from, int c, F2 (&v)[4]) {
     if (VEC) take8<T, CH>(stage, array, c, v);
+    else if (MODE == kShifted) take_shifted8<T>(stage + array * span + row_low(from), group_column(c, off), H, v);
     else take_span8<T>(stage + array * span + row_low(from), c, H, v);
     if (MODE == kEdges && partial(group_column(c, off), H)) clip8(group_column(c, off), H, v);
   };
-  if (MODE == kEdges) {                            // the parameters at the thread's columns, behind the ring
+  if (has_edges(MODE)) {                           // the parameters at the thread's columns, behind the ring
     const void* const from[3] = {a.pre_w, a.post_w, gate_kind == kGateChannel ? a.gate : nullptr};
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
@@ -550,17 +576,17 @@ __global__ void __launch_bounds__(kNormThreads) block_norm_backward_kernel(NormA
 // rows come through a ring like the forward's, the column sums stay in registers as fp32, and the weights, which leave no
 // registers for themselves, in shared memory behind the ring (an SM's quarter has 128 registers for each of four warps).
 // Missing parts are neutral values (y = 0, w_post = 1, gate = 1) instead of branches.
-template <typename T, int CH, int MODE, int GATE>
-__global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 2 : 1) block_norm_backward_ring_kernel(NormArgs a) {
+template <typename T, int CH, RowMode MODE, int GATE>
+__global__ void __launch_bounds__(kNormThreads) block_norm_backward_ring_kernel(NormArgs a) {
   griddep_launch_dependents();
   griddep_wait();
-  constexpr bool VEC = MODE != kSpan;
+  constexpr bool VEC = by_block(MODE);
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float red[2][96];
   const int H = a.H;
   const float inv_h = 1.0f / static_cast<float>(H), scale = a.y ? a.a : 1.0f;
   const int span = span_bytes(H, sizeof(T));
-  const int off = MODE == kEdges ? static_cast<int>(blockIdx.x * static_cast<int64_t>(H) % (16 / static_cast<int>(sizeof(T)))) : 0;
+  const int off = has_edges(MODE) ? static_cast<int>(blockIdx.x * static_cast<int64_t>(H) % (16 / static_cast<int>(sizeof(T)))) : 0;
   const uint32_t stage_bytes = static_cast<uint32_t>(a.arrays * (VEC ? CH * blockDim.x * sizeof(Pack8<T>) : span));
   auto fetch_one = [&](uint32_t stage, int array, const void* p, int64_t at) {
     if (VEC) fetch_row<T, CH, MODE>(stage, array, static_cast<const T*>(p) + at, H, off);
@@ -583,7 +609,7 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 2 : 1)
 
   auto take = [&](const uint8_t* stage, int array, const void* p, int64_t at, int c, F2 (&v)[4]) {
     if (VEC) take8<T, CH>(stage, array, c, v);
-    else if (p) take_span8<T>(stage + array * span + row_low(static_cast<const T*>(p) + at), c, H, v);
+    else if (p) take_shifted8<T>(stage + array * span + row_low(static_cast<const T*>(p) + at), group_column(c, off), H, v);
     else v[0] = v[1] = v[2] = v[3] = both(0.0f);
     if (MODE == kEdges && partial(group_column(c, off), H)) clip8(group_column(c, off), H, v);
   };
@@ -596,8 +622,8 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 2 : 1)
     for (int k = 0; k < (GATE == kGateChannel ? 3 : 2); ++k) {
       F2 w[4] = {both(1.0f), both(1.0f), both(1.0f), both(1.0f)};
       if (from[k]) {
-        if (MODE == kEdges) load8_at<T>(static_cast<const T*>(from[k]), group_column(c, off), H, 1.0f, w);
-        else load8<T, VEC>(static_cast<const T*>(from[k]), c, H, w);
+        if (has_edges(MODE)) load8_at<T>(static_cast<const T*>(from[k]), group_column(c, off), H, 1.0f, w);
+        else load8<T, true>(static_cast<const T*>(from[k]), c, H, w);
       }
       put8<T, CH>(weights, k, c, w);
     }
@@ -753,6 +779,13 @@ Shape shape_of(int H) {
   return {ch, ((groups + ch - 1) / ch + 31) / 32 * 32};
 }
 
+// The backward kernels hold more per column: one group a thread up to 512 threads.
+Shape backward_shape_of(int H) {
+  const int groups = (H + 7) / 8;
+  const int ch = groups <= kNormThreads ? 1 : groups <= 2 * kNormThreads ? 2 : 4;
+  return {ch, ((groups + ch - 1) / ch + 31) / 32 * 32};
+}
+
 // How the rows of this call can be moved; for kEdges parameters need the activations' type too.
 RowMode row_mode(const NormArgs& a, int dtype) {
   const int size = element_size(dtype), block = 16 / size;
@@ -761,23 +794,25 @@ RowMode row_mode(const NormArgs& a, int dtype) {
       {a.s, a.H, size}, {a.h, a.H, size}, {a.dx, a.H, size}, {a.dy, a.H, size},
       {a.gate_kind == kGateFull ? a.gate : nullptr, a.gate_stride, a.gate_f32 ? 4 : size},
       {a.gate_kind == kGateFull ? a.dgate_rows : nullptr, a.H, a.gate_f32 ? 4 : size}};
-  bool all = a.H % 8 == 0, congruent = true;
+  bool all = a.H % 8 == 0, congruent = true, results = true;
   for (const auto& r : rows) {
-    if (!r.p || aligned(r.p, 16)) {
-      all = all && (!r.p || r.stride * r.size % 16 == 0);
-      congruent = congruent && (!r.p || ((r.stride - a.H) % block == 0 && r.size == size));
-    } else {
-      all = congruent = false;
-    }
+    if (!r.p) continue;
+    const bool base = aligned(r.p, 16);
+    all = all && base && r.stride * r.size % 16 == 0;
+    congruent = congruent && base && (r.stride - a.H) % block == 0 && r.size == size;
   }
+  for (const void* p : {static_cast<const void*>(a.s), static_cast<const void*>(a.h), static_cast<const void*>(a.dx),
+                        static_cast<const void*>(a.dy), a.gate_kind == kGateFull ? static_cast<const void*>(a.dgate_rows) : nullptr})
+    results = results && aligned(p, 16);
   const bool params = aligned(a.pre_w, 16) && aligned(a.post_w, 16) && (a.gate_kind != kGateChannel || aligned(a.gate, 16));
   if (all && params && aligned(a.q, 8)) return kAligned;
   const bool own_type = size == 4 || !(a.pre_f32 || a.post_f32 || a.gate_f32);
-  return congruent && own_type && !a.q && shape_of(a.H + 7).ch <= 2 ? kEdges : kSpan;
+  if (!own_type || a.q || !results || shape_of(a.H + 7).ch > 2) return kSpan;
+  return congruent ? kEdges : kShifted;
 }
 
-// Width by which threads are counted: with kEdges a row has up to one block more.
-int counted_width(int H, RowMode mode) { return mode == kEdges ? H + 7 : H; }
+// Width by which threads are counted: with edges a row has up to one block more.
+int counted_width(int H, RowMode mode) { return has_edges(mode) ? H + 7 : H; }
 
 bool bad_common(const NormArgs& a, int dtype, int param_f32) {
   if (dtype < MOE_B200_F32 || dtype > MOE_B200_F16) return true;
@@ -792,11 +827,12 @@ bool bad_common(const NormArgs& a, int dtype, int param_f32) {
          (a.post_w && !a.y);
 }
 
+constexpr size_t kSmemMost = 224 * 1024;          // dynamic shared memory a kernel here may have
 constexpr size_t kRingMost = 208 * 1024;          // shared memory of an SM for rings; the rest is first-level cache
 
 int grid_rows(int T, int per_sm, RowMode mode) {
   if (T <= kNumSMs * per_sm) return T;
-  return mode == kEdges ? kNumSMs * per_sm / 8 * 8 : kNumSMs * per_sm;
+  return has_edges(mode) ? kNumSMs * per_sm / 8 * 8 : kNumSMs * per_sm;
 }
 
 // Activations that a row's ring stage holds: x, y and a full gate of the same type.
@@ -808,8 +844,8 @@ template <typename T, int CH, RowMode MODE, bool QUANT, int GATE>
 cudaError_t launch_forward(NormArgs a, int threads, cudaStream_t stream) {
   const auto kernel = block_norm_kernel<T, CH, MODE, QUANT, GATE>;
   a.arrays = forward_arrays(a, sizeof(T));
-  const size_t stage = static_cast<size_t>(a.arrays) * (MODE != kSpan ? CH * threads * sizeof(Pack8<T>) : span_bytes(a.H, sizeof(T)));
-  const size_t weights = MODE == kEdges ? 3 * CH * threads * sizeof(Pack8<T>) : 0;
+  const size_t stage = static_cast<size_t>(a.arrays) * (by_block(MODE) ? CH * threads * sizeof(Pack8<T>) : span_bytes(a.H, sizeof(T)));
+  const size_t weights = has_edges(MODE) ? 3 * CH * threads * sizeof(Pack8<T>) : 0;
   // as many CTAs as the registers are cut for, or fewer where their rings do not fit; two stages at least, if that can be
   // had
   int per_sm = 896 / threads > 0 ? 896 / threads : 1;
@@ -817,7 +853,8 @@ cudaError_t launch_forward(NormArgs a, int threads, cudaStream_t stream) {
   a.ring = static_cast<int>((kRingMost / per_sm - weights) / stage);
   if (a.ring > kMaxRing) a.ring = kMaxRing;
   const size_t smem = a.ring * stage + weights;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(kernel, kSmemMost, done);
   if (e != cudaSuccess) return e;
   return launch_pdl(kernel, dim3(grid_rows(a.T, per_sm, MODE)), dim3(threads), smem, stream, a);
 }
@@ -834,6 +871,7 @@ template <typename T, int CH>
 cudaError_t launch_forward(const NormArgs& a, RowMode mode, bool known, int threads, cudaStream_t stream) {
   constexpr int kCh = CH <= 2 ? CH : 1;
   if (mode == kEdges) return launch_forward<T, kCh, kEdges, false>(a, threads, stream);
+  if (mode == kShifted) return launch_forward<T, kCh, kShifted, false>(a, threads, stream);
   if (mode == kSpan) return launch_forward<T, CH, kSpan, false, kAnyGate>(a, threads, stream);
   if (known) return a.q ? launch_forward<T, kCh, kAligned, true>(a, threads, stream) : launch_forward<T, kCh, kAligned, false>(a, threads, stream);
   return a.q ? launch_forward<T, CH, kAligned, true, kAnyGate>(a, threads, stream)
@@ -851,15 +889,15 @@ cudaError_t launch_forward(const NormArgs& a, RowMode mode, cudaStream_t stream)
 
 // CTAs of the backward pass, one partial row of column sums each: as many as the registers hold.
 int backward_parts(int T, int H, RowMode mode) {
-  const Shape sh = shape_of(counted_width(H, mode));
+  const Shape sh = backward_shape_of(counted_width(H, mode));
   return grid_rows(T, sh.ch > 1 ? 1 : 512 / sh.threads, mode);
 }
 
 template <typename T, int CH, bool VEC>
 cudaError_t launch_backward(const NormArgs& a, int grid, int threads, cudaStream_t stream) {
   const size_t smem = static_cast<size_t>(a.n_sums) * CH * 8 * threads * sizeof(float);
-  const cudaError_t e = cudaFuncSetAttribute(block_norm_backward_kernel<T, CH, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(smem));
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(block_norm_backward_kernel<T, CH, VEC>, kSmemMost, done);
   if (e != cudaSuccess) return e;
   return launch_pdl(block_norm_backward_kernel<T, CH, VEC>, dim3(grid), dim3(threads), smem, stream, a);
 }
@@ -867,11 +905,11 @@ cudaError_t launch_backward(const NormArgs& a, int grid, int threads, cudaStream
 // Whether the ring kernel takes this call (a longer row or a mixed call goes to the other one), its stages and memory.
 template <typename T>
 bool ring_plan(NormArgs& a, RowMode mode, size_t* smem) {
-  const Shape sh = shape_of(counted_width(a.H, mode));
-  if (sh.ch > 2 || (sizeof(T) == 2 && (a.pre_f32 || a.post_f32 || a.gate_f32))) return false;
+  const Shape sh = backward_shape_of(counted_width(a.H, mode));
+  if (mode == kSpan || sh.ch > 2 || (sizeof(T) == 2 && (a.pre_f32 || a.post_f32 || a.gate_f32))) return false;
   a.arrays = a.gate_kind == kGateFull ? 5 : 4;
   const size_t array = static_cast<size_t>(sh.ch) * sh.threads * sizeof(Pack8<T>), weights = 3 * array;
-  const size_t stage = a.arrays * (mode != kSpan ? array : span_bytes(a.H, sizeof(T)));
+  const size_t stage = a.arrays * (by_block(mode) ? array : span_bytes(a.H, sizeof(T)));
   const size_t room = 220 * 1024 / (sh.ch == 1 ? 512 / sh.threads : 1) - 2048;
   a.ring = room > weights ? static_cast<int>((room - weights) / stage) : 0;
   if (a.ring > kMaxRing) a.ring = kMaxRing;
@@ -887,7 +925,8 @@ bool ring_fits(NormArgs a, RowMode mode) {
 template <typename T, int CH, RowMode MODE, int GATE>
 cudaError_t launch_ring(const NormArgs& a, int grid, int threads, size_t smem, cudaStream_t stream) {
   const auto kernel = block_norm_backward_ring_kernel<T, CH, MODE, GATE>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(kernel, kSmemMost, done);
   if (e != cudaSuccess) return e;
   return launch_pdl(kernel, dim3(grid), dim3(threads), smem, stream, a);
 }
@@ -903,13 +942,13 @@ template <typename T, int CH>
 cudaError_t launch_ring(const NormArgs& a, RowMode mode, int grid, int threads, size_t smem, cudaStream_t stream) {
   if (mode == kAligned) return launch_ring<T, CH, kAligned>(a, grid, threads, smem, stream);
   if (mode == kEdges) return launch_ring<T, CH, kEdges>(a, grid, threads, smem, stream);
-  return launch_ring<T, CH, kSpan>(a, grid, threads, smem, stream);
+  return launch_ring<T, CH, kShifted>(a, grid, threads, smem, stream);
 }
 
 template <typename T>
 cudaError_t launch_backward(NormArgs a, ColumnSumArgs cs, RowMode mode, cudaStream_t stream) {
-  if (mode == kEdges && !ring_fits<T>(a, mode)) mode = kSpan;
-  const Shape sh = shape_of(counted_width(a.H, mode));
+  if (has_edges(mode) && !ring_fits<T>(a, mode)) mode = kSpan;
+  const Shape sh = backward_shape_of(counted_width(a.H, mode));
   cs.n_parts = backward_parts(a.T, a.H, mode);
   const int grid = cs.n_parts, nt = sh.threads;
   size_t smem = 0;
@@ -967,7 +1006,7 @@ extern "C" int moe_fp8_block_scale_block_norm(const void* x, int64_t x_stride, c
 extern "C" size_t moe_fp8_block_scale_block_norm_backward_workspace_bytes(int T, int H) {
   if (T < 0 || H < 1 || H > kMaxWidth) return 0;
   int parts = 0;
-  for (RowMode mode : {kSpan, kAligned, kEdges}) {
+  for (RowMode mode : {kSpan, kEdges}) {
     const int n = backward_parts(T, H, mode);
     parts = n > parts ? n : parts;
   }

@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "../../include/moe_b200.h"
 #include "kernels.h"
 
@@ -17,6 +19,19 @@ inline int launch_status(cudaError_t e, int launches) {
   }
   count_launches(launches);
   return MOE_B200_OK;
+}
+// Lets `kernel` have up to `bytes` of dynamic shared memory on the current device; `done` (a static of the caller, one per
+// kernel) remembers the devices where that has been said, a driver call that would cost a small launch a tenth of its time.
+template <typename Kernel>
+inline cudaError_t allow_smem(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = uint64_t(1) << (device & 63);
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e == cudaSuccess && device < 64) done.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 inline int element_size(int dtype) { return dtype == MOE_B200_F32 ? 4 : 2; }
 inline bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }

@@ -486,7 +486,8 @@ cudaError_t launch_kernel(MatvecArgs a, cudaStream_t stream) {
   a.slice_steps = slice;
   a.x_row = slice * (kStep / 8) + 4;                 // rows 64 bytes apart in the banks
   const size_t smem = kRing + static_cast<size_t>(a.x_cols) * a.x_row * 16 + kStep * 2 + static_cast<size_t>(slice) * (kStep / G) * 8 * NT * 4;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kRing + kX + kStep * 2));
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(kernel, kRing + kX + kStep * 2, done);
   if (e != cudaSuccess) return e;
   const int64_t most = static_cast<int64_t>((a.N + kTile - 1) / kTile) * a.pairs;
   return launch_pdl(kernel, dim3(static_cast<unsigned>(most < kNumSMs ? most : kNumSMs)), dim3(kThreads), smem, stream, a);
