@@ -47,8 +47,8 @@ struct MatvecArgs {
   const int* experts;        // [pairs] or null
   int pairs, per_row, E, N, K, scale_f32, out_f32;
   int x_cols;                // rows of x that are staged at most
-  int slice_steps;           // steps of 256 columns staged at a time
-  int x_row;                 // 16-byte chunks between staged rows
+  int slice_most;            // steps of 256 columns staged at a time at most
+  int x_chunks;              // 16-byte chunks for staged x: a job with fewer rows stages more steps at a time
   void* out;                 // [pairs, N]
 };
 
@@ -223,6 +223,7 @@ struct Cursor {
   int job, round, slice, u, end;
   int tile, tile_end;        // first tile of the CTA's run in this job and the one behind its last
   int lw;                    // log2 of the warps that share an item of the run
+  int slice_steps, slices;   // of x
 };
 
 // G: group size.  NT: token tiles of eight columns.  ZERO: a table of zero points.
@@ -234,14 +235,14 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
   __shared__ float red[2][kWarps][kCols][kTile + 4];
   __shared__ Jobs jobs;
   __shared__ int scan[kWarps];
-  __shared__ const T* x_row[kCols];
+  __shared__ const T* x_from[kCols];
   static_assert(sizeof(red) >= kMaxMatvecExperts * sizeof(int), "find_jobs' table lies in red");
   griddep_launch_dependents();
   griddep_wait();
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, quad = lane & 3;
   uint4* const xs = reinterpret_cast<uint4*>(smem + kWarps * kDepth * S::kBytes);
-  uint4* const none = xs + a.x_cols * a.x_row;     // what lanes without a column multiply
+  uint4* const none = xs + a.x_chunks;             // what lanes without a column multiply
   float* const xsum = reinterpret_cast<float*>(none + kStep / 8);   // [groups of a slice][kCols]
   const uint32_t ring = smem_address(smem) + warp * kDepth * S::kBytes;
   if (tid < kStep / 8) none[tid] = make_uint4(0u, 0u, 0u, 0u);
@@ -255,7 +256,6 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
   }
 
   const int steps = (a.K + kStep - 1) / kStep, groups = a.K / G, tiles = (a.N + kTile - 1) / kTile;
-  const int slices = (steps + a.slice_steps - 1) / a.slice_steps;
   const int64_t items = static_cast<int64_t>(jobs.n) * tiles;
   // The CTA's run of items.  A run that goes on into the next job stages x twice and ends two rounds with idle warps, so
   // with few jobs every CTA stays in one of them; with many, equal runs matter more.
@@ -273,6 +273,8 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
   const int last_job = (item1 - 1) / tiles;
 
   auto open_job = [&](Cursor& c) {
+    c.slice_steps = min(a.slice_most, (a.x_chunks / jobs.cols[c.job] - 4) / (kStep / 8));
+    c.slices = (steps + c.slice_steps - 1) / c.slice_steps;
     c.tile = max(item0 - c.job * tiles, 0);
     c.tile_end = min(item1 - c.job * tiles, tiles);
     // the fewest steps until the last warp is done with the run, with about a step's time for a join
@@ -288,13 +290,13 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
   };
   auto tile_of = [&](const Cursor& c) { return c.tile + (c.round << (kLogWarps - c.lw)) + (warp >> c.lw); };
   auto open = [&](Cursor& c) {                     // the warp's steps in (job, round, slice)
-    const int s0 = c.slice * a.slice_steps, s1 = min(steps, s0 + a.slice_steps), per = (s1 - s0 + (1 << c.lw) - 1) >> c.lw;
+    const int s0 = c.slice * c.slice_steps, s1 = min(steps, s0 + c.slice_steps), per = (s1 - s0 + (1 << c.lw) - 1) >> c.lw;
     c.u = min(s1, s0 + (warp & ((1 << c.lw) - 1)) * per);
     c.end = tile_of(c) < c.tile_end ? min(s1, c.u + per) : c.u;
   };
 
   // ---- loads, which run kDepth steps ahead
-  Cursor ld = {item0 / tiles, 0, 0, 0, 0, 0, 0, 0};
+  Cursor ld = {item0 / tiles, 0, 0, 0, 0, 0, 0, 0, 0, 0};
   const int row8 = lane >> 3, chunk8 = lane & 7;   // a copy instruction takes four rows of 128 bytes
   const uint8_t* ld_q[4];                          // the lane's chunk of rows row8, row8 + 4, ...
   uintptr_t ld_s, ld_z;                            // scales and zeros of row lane % 16
@@ -314,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
   };
   auto load = [&](uint32_t stage) {
     while (ld.u >= ld.end && ld.job <= last_job) {
-      if (++ld.slice == slices) {
+      if (++ld.slice == ld.slices) {
         ld.slice = 0;
         ++ld.round;
         if (ld.tile + (ld.round << (kLogWarps - ld.lw)) >= ld.tile_end) {
@@ -362,10 +364,11 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
 
   // ---- products
   int slot = 0, par = 0;
-  Cursor at = {item0 / tiles, 0, 0, 0, 0, 0, 0, 0};
+  Cursor at = {item0 / tiles, 0, 0, 0, 0, 0, 0, 0, 0, 0};
   for (; at.job <= last_job; ++at.job) {
     open_job(at);
     const int cols = jobs.cols[at.job], first = jobs.first[at.job], wk = 1 << at.lw, at_once = kWarps >> at.lw;
+    const int x_row = at.slice_steps * (kStep / 8) + 4;   // 16-byte chunks between staged rows: 64 bytes apart in the banks
     for (at.round = 0; at.tile + at.round * at_once < at.tile_end; ++at.round) {
       const int n0 = tile_of(at) * kTile;
       float sum[NT][4];
@@ -374,23 +377,23 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[t][i] = 0.0f;
 
-      for (at.slice = 0; at.slice < slices; ++at.slice) {
-        const int s0 = at.slice * a.slice_steps, s1 = min(steps, s0 + a.slice_steps);
-        if (at.round == 0 || slices > 1) {
+      for (at.slice = 0; at.slice < at.slices; ++at.slice) {
+        const int s0 = at.slice * at.slice_steps, s1 = min(steps, s0 + at.slice_steps);
+        if (at.round == 0 || at.slices > 1) {
           // stage x: a 16-byte chunk holds eight k, stored as the pairs (0, 4), (2, 6), (1, 5), (3, 7); chunk j of quad
           // lane t of a group lies at 4 j + t
           __syncthreads();
           const int chunks = (s1 - s0) * (kStep / 8), held = (min(a.K, s1 * kStep) - s0 * kStep) / 8;   // zeros behind K
           if (tid < cols)
-            x_row[tid] = static_cast<const T*>(a.x) + (jobs.list[first + tid] / a.per_row) * a.x_stride + static_cast<int64_t>(s0) * kStep;
+            x_from[tid] = static_cast<const T*>(a.x) + (jobs.list[first + tid] / a.per_row) * a.x_stride + static_cast<int64_t>(s0) * kStep;
           __syncthreads();
           for (int i = tid; i < chunks; i += kThreads) {
             const int in = i % (G / 8), to = i - in + (in % W) * 4 + in / W;
 #pragma unroll 4
             for (int c = 0; c < cols; ++c) {
               uint4 v = make_uint4(0u, 0u, 0u, 0u);
-              if (i < held) v = __ldg(reinterpret_cast<const uint4*>(x_row[c]) + i);
-              xs[c * a.x_row + to] =
+              if (i < held) v = __ldg(reinterpret_cast<const uint4*>(x_from[c]) + i);
+              xs[c * x_row + to] =
                   make_uint4(Mma<T>::staged(__byte_perm(v.x, v.z, 0x5410)), Mma<T>::staged(__byte_perm(v.y, v.w, 0x5410)),
                              Mma<T>::staged(__byte_perm(v.x, v.z, 0x7632)), Mma<T>::staged(__byte_perm(v.y, v.w, 0x7632)));
               const float2 p = Mma<T>::widen(v.x), q = Mma<T>::widen(v.y), r = Mma<T>::widen(v.z), t = Mma<T>::widen(v.w);
@@ -419,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const bool has = 8 * t + gid < cols;
-          x_at[t] = reinterpret_cast<const uint8_t*>((has ? xs + (8 * t + gid) * a.x_row + (at.u - s0) * (kStep / 8) : none) + quad);
+          x_at[t] = reinterpret_cast<const uint8_t*>((has ? xs + (8 * t + gid) * x_row + (at.u - s0) * (kStep / 8) : none) + quad);
           x_step[t] = has ? 2 * kStep : 0;
         }
         for (; at.u < at.end; ++at.u) {
@@ -480,17 +483,20 @@ cudaError_t launch_kernel(MatvecArgs a, cudaStream_t stream) {
   const int rows = a.pairs / a.per_row;             // a row that names an expert twice gives it a second job
   a.x_cols = rows < 8 * NT ? rows : 8 * NT;
   const int steps = (a.K + kStep - 1) / kStep;
-  const size_t per_step = static_cast<size_t>(a.x_cols) * kStep * 2 + kStep / G * 8 * NT * 4;
-  int slice = static_cast<int>((kX - a.x_cols * 64) / per_step);
-  if (slice > steps) slice = steps;
-  a.slice_steps = slice;
-  a.x_row = slice * (kStep / 8) + 4;                 // rows 64 bytes apart in the banks
-  const size_t smem = kRing + static_cast<size_t>(a.x_cols) * a.x_row * 16 + kStep * 2 + static_cast<size_t>(slice) * (kStep / G) * 8 * NT * 4;
+  // steps that fit for one row, the sums of their groups, and the rest for staged rows, as much of it as the call can use
+  constexpr size_t kSums = static_cast<size_t>(kStep / G) * 8 * NT * 4;
+  const int most = static_cast<int>((kX - 64) / (kStep * 2 + kSums));
+  a.slice_most = steps < most ? steps : most;
+  size_t room = kX - a.slice_most * kSums;
+  const size_t useful = static_cast<size_t>(a.x_cols) * (a.slice_most * kStep * 2 + 64);
+  if (room > useful) room = useful;
+  a.x_chunks = static_cast<int>(room / 16);
+  const size_t smem = kRing + static_cast<size_t>(a.x_chunks) * 16 + kStep * 2 + a.slice_most * kSums;
   static std::atomic<uint64_t> done{0};
   const cudaError_t e = allow_smem(kernel, kRing + kX + kStep * 2, done);
   if (e != cudaSuccess) return e;
-  const int64_t most = static_cast<int64_t>((a.N + kTile - 1) / kTile) * a.pairs;
-  return launch_pdl(kernel, dim3(static_cast<unsigned>(most < kNumSMs ? most : kNumSMs)), dim3(kThreads), smem, stream, a);
+  const int64_t items = static_cast<int64_t>((a.N + kTile - 1) / kTile) * a.pairs;
+  return launch_pdl(kernel, dim3(static_cast<unsigned>(items < kNumSMs ? items : kNumSMs)), dim3(kThreads), smem, stream, a);
 }
 
 template <typename T, int NT>
