@@ -513,8 +513,10 @@ cudaError_t launch_group(const MatvecArgs& a, int G, cudaStream_t stream) {
 
 template <typename T>
 cudaError_t launch_matvec(const MatvecArgs& a, int G, cudaStream_t stream) {
-  // one tile of eight columns where no expert can have more rows (a row chooses an expert once)
-  return a.pairs / a.per_row <= 8 ? launch_group<T, 1>(a, G, stream) : launch_group<T, 2>(a, G, stream);
+  // One tile of eight columns where no expert can have more rows (a row chooses an expert once), and where at most four of
+  // them are expected: an expert that has more all the same is read twice.
+  const bool one = a.pairs / a.per_row <= 8 || (a.experts && a.pairs <= 4 * a.E);
+  return one ? launch_group<T, 1>(a, G, stream) : launch_group<T, 2>(a, G, stream);
 }
 
 }  // namespace
