@@ -426,7 +426,7 @@ cudaError_t launch_balance(const BalanceArgs& a, int dtype, bool backward, cudaS
 }
 
 bool bad_common(int T, int E, int K, int S, int dtype, int scoring, const int32_t* cu_seqlens) {
-  return T < 0 || E < 1 || E > kMaxExperts || K < 1 || K > E || S < 0 || (!cu_seqlens && S != 1) || dtype < MOE_B200_F32 ||
+  return T < 0 || T > (1 << 30) || S > (1 << 30) || E < 1 || E > kMaxExperts || K < 1 || K > E || S < 0 || (!cu_seqlens && S != 1) || dtype < MOE_B200_F32 ||
          dtype > MOE_B200_F16 || scoring < MOE_B200_SCORE_SIGMOID || scoring > MOE_B200_SCORE_SOFTMAX;
 }
 

@@ -21,6 +21,7 @@ namespace moe {
 namespace {
 
 constexpr int kMaxWidth = 16384;
+constexpr int kMostTokens = 1 << 30;       // row indexes and a grid's step stay within an int
 constexpr int kNormThreads = 512;
 
 enum GateKind : int { kGateNone = 0, kGateChannel = 1, kGateToken = 2, kGateFull = 3 };
@@ -426,7 +427,8 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 3 : CH
         for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fmaxf(fabsf(get(s[c][j]).x), fabsf(get(s[c][j]).y)));
 #pragma unroll
         for (int d = 8; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
-        const F2 inverse = both(__fdividef(448.0f, amax));
+        const float scale = amax * (1.0f / 448.0f);
+        const F2 inverse = both(__fdividef(1.0f, scale));
         uint32_t packed[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -434,7 +436,7 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 3 : CH
                       static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(get(mul2(s[c][2 * j + 1], inverse)), __NV_SATFINITE, __NV_E4M3)) << 16;
         if (col < H) {
           *reinterpret_cast<uint2*>(q_out + col) = make_uint2(packed[0], packed[1]);
-          if ((threadIdx.x & 15) == 0) a.q_scale[static_cast<int64_t>(col / kBlock) * a.T + row] = amax * (1.0f / 448.0f);
+          if ((threadIdx.x & 15) == 0) a.q_scale[static_cast<int64_t>(col / kBlock) * a.T + row] = scale;
         }
       } else {
         store_row8<T, MODE>(h_out, c, H, off, s[c]);
@@ -822,7 +824,7 @@ bool bad_common(const NormArgs& a, int dtype, int param_f32) {
     if (!aligned(p, size)) return true;
   if (!aligned(a.pre_w, a.pre_f32 ? 4 : size) || !aligned(a.post_w, a.post_f32 ? 4 : size) || !aligned(a.gate, a.gate_f32 ? 4 : size))
     return true;
-  return a.T < 0 || a.H < 1 || a.H > kMaxWidth || (param_f32 & ~7) ||
+  return a.T < 0 || a.T > kMostTokens || a.H < 1 || a.H > kMaxWidth || (param_f32 & ~7) ||
          a.gate_kind < kGateNone || a.gate_kind > kGateFull || (a.gate_kind != kGateNone && (!a.gate || !a.y)) ||
          (a.post_w && !a.y);
 }

@@ -98,6 +98,7 @@ struct Jobs {
   int list[kMaxPairs];       // pairs, by expert in order of first appearance, ascending inside
   int expert[kMaxPairs], first[kMaxPairs], cols[kMaxPairs];   // of a job: its expert, first entry of list, entries
   int n;
+  uint32_t missing[kMaxPairs / 32];   // pairs whose expert is not held here
 };
 
 // Fills `jobs` from experts[]; every CTA does it for itself (a few hundred cycles).  `table` has an entry per expert.
@@ -107,6 +108,10 @@ __device__ __forceinline__ void find_jobs(const MatvecArgs& a, int max_cols, Job
   if (tid < a.pairs) e = a.experts ? a.experts[tid] : 0;
   const bool held = e >= 0 && e < a.E;
   if (held) table[e] = 0;
+  if (warp < kMaxPairs / 32) {
+    const uint32_t none = __ballot_sync(0xFFFFFFFFu, tid < a.pairs && !held);
+    if (lane == 0) jobs.missing[warp] = none;
+  }
   __syncthreads();
   // place among the pairs of the same expert: warp after warp, so that the order is the pairs' own
   const uint32_t peers = __match_any_sync(0xFFFFFFFFu, held ? e : -1);
@@ -247,10 +252,9 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
   const uint32_t ring = smem_address(smem) + warp * kDepth * S::kBytes;
   if (tid < kStep / 8) none[tid] = make_uint4(0u, 0u, 0u, 0u);
   find_jobs(a, a.x_cols, jobs, reinterpret_cast<int*>(red), scan);
-  if (a.experts) {
-    for (int p = 0; p < a.pairs; ++p) {
-      const int e = a.experts[p];
-      if (e >= 0 && e < a.E) continue;
+  for (int w = 0; w < kMaxPairs / 32; ++w) {
+    for (uint32_t left = jobs.missing[w]; left != 0; left &= left - 1) {
+      const int p = w * 32 + __ffs(left) - 1;
       for (int n = blockIdx.x * kThreads + tid; n < a.N; n += gridDim.x * kThreads) store_result<T>(a, p, n, 0.0f);
     }
   }

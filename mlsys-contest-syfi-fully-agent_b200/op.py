@@ -311,8 +311,8 @@ def _norm_inputs(x, pre_weight, y, post_weight, gate, residual_scale):
     if code is None or len(shape) != 2:
         raise ValueError("x must be float32, bfloat16 or float16 [T, H]")
     T, H = shape
-    if not 1 <= H <= NORM_MAX_WIDTH or T >= 2 ** 31:
-        raise ValueError(f"x must have 1 to {NORM_MAX_WIDTH} columns")
+    if not 1 <= H <= NORM_MAX_WIDTH or T > 2 ** 30:
+        raise ValueError(f"x must have at most 2^30 rows and 1 to {NORM_MAX_WIDTH} columns")
     xp, xs = _rows("x", x, shape, dtype, dev)
     pre, f32 = _param("pre_weight", pre_weight, H, dtype, dev)
     params = 1 if f32 else 0
@@ -416,8 +416,8 @@ def _balance_inputs(logits, top_k, cu_seqlens, token_mask, scoring):
     if code is None or len(shape) != 2:
         raise ValueError("logits must be float32, bfloat16 or float16 [T, E]")
     T, E = shape
-    if not 1 <= E <= BALANCE_MAX_EXPERTS or T >= 2 ** 31:
-        raise ValueError(f"logits must have 1 to {BALANCE_MAX_EXPERTS} columns")
+    if not 1 <= E <= BALANCE_MAX_EXPERTS or T > 2 ** 30:
+        raise ValueError(f"logits must have at most 2^30 rows and 1 to {BALANCE_MAX_EXPERTS} columns")
     if E > 1 and logits.stride(1) != 1:
         raise ValueError("logits: the elements of a row must be adjacent")
     if not 1 <= top_k <= E:

@@ -109,6 +109,10 @@ NORM = [
     (900, 2304, BF, "token", True, True, 3, 2, False),
     (1500, 770, HF, "none", False, False, 0, 0, False),
     (2500, 640, BF, "full", True, True, 0, 0, False),
+    (1, 1001, BF, "channel", True, True, 0, 0, False),
+    (2, 517, F, "token", True, True, 0, 3, False),
+    (500, 6001, HF, "full", True, True, 3, 0, False),
+    (340, 4104, BF, "channel", True, True, 5, 0, False),
     (620, 7168, BF, "full", True, False, 8, 0, False),
 ]
 
@@ -256,6 +260,17 @@ def test_block_norm_quantized_zero_rows(op):
     assert not bool(q.to(F).any())
     floor = torch.full_like(scale, 1e-10, dtype=D) / 448
     near(scale, floor, floor)
+
+
+def test_block_norm_quantized_near_the_largest_values(op):
+    """h up to 3e38: the scale stays finite and the largest value of a block is 448 steps of it."""
+    x = torch.ones((2, 256), device="cuda")
+    w = torch.full((256,), 3e38, device="cuda")
+    w[128:] = 1e-20
+    q, scale = op.block_norm(x, w, quantize=True)[1]
+    assert bool((q[:, :128].to(F) == 448).all()) and bool(torch.isfinite(scale).all())
+    assert abs(float(scale[0, 0]) * 448 / 3e38 - 1) < 1e-5
+    assert not bool(q[:, 128:].to(F).any())               # 1e-20 over the floor of 1e-10 / 448
 
 
 # ---------------------------------------------------------------------------- balance loss
@@ -429,6 +444,10 @@ MATVEC = [
     (17, 48, 1152, 128, BF, True, None, 0, None),
     (100, 40, 640, 64, BF, False, None, 0, None),
     (256, 19, 256, 128, HF, False, None, 0, None),
+    # more columns than are staged at a time
+    (16, 40, 20480, 128, BF, False, None, 0, None),
+    (3, 24, 65536, 64, HF, True, None, 0, F),
+    (11, 33, 19232, 32, BF, True, None, 0, None),
 ]
 
 
@@ -449,6 +468,9 @@ def test_matvec(op, g, R, N, K, G, t, zero, st, pad, ot):
     (16, 16, 2, 40, 256, 64, BF, True, False, 1),          # every pair on one expert
     (13, 3, 7, 130, 384, 128, HF, False, True, 7),
     (256, 1, 5, 17, 128, 128, BF, False, True, 6),
+    (16, 8, 32, 100, 1024, 128, BF, False, False, 3),      # more rows on an expert than the batch's size makes likely
+    (3, 4, 2, 70, 512, 64, HF, False, False, 1),           # an expert named more than once by a row
+    (9, 2, 1000, 33, 256, 32, BF, True, True, 1200),
 ])
 def test_matvec_by_experts(op, g, T, k, E, N, K, G, t, zero, per_pair, span):
     x, q, scale, z = matvec_inputs(g, T * k if per_pair else T, N, K, G, t, E, zero)
