@@ -7,7 +7,8 @@ The directory name is not a Python identifier; load it with
 Sub-modules:
   gen     seeded synthetic workloads
   loader  ctypes binding of the C-ABI library (fails loudly if it is missing)
-  op      ``run(...)`` with the reference entry point's argument list
+  op      ``run(...)`` with the reference entry point's argument list; routing, quantisation; block norms, balance loss and
+          4-bit matrix-vector products for the steps around the shard
   ep      expert-parallel 256-expert layer over torch.distributed
   build   nvcc build of csrc/ for sm_100a
   packaging  config.toml + solution.json in the reference's schema

@@ -20,7 +20,7 @@ LIB_TVMFFI = os.path.join(HERE, "libmoe_b200_tvmffi.so")
 SOURCES = ["launcher.cu", "route_permute.cu", "grouped_gemm.cu", "grouped_gemm_large.cu", "decode_kernel.cu", "swiglu_combine.cu", "static_entry.cu", "quantize.cu", "ep_push.cu", "block_norm.cu", "balance_loss.cu", "matvec_w4.cu"]
 HEADERS = ["kernels.h", "moe_layout.h", "ptx.cuh", "route_device.cuh", "epilogue_device.cuh", "gemm_common.cuh", "map_cache.h", "elem_device.cuh", os.path.join("..", "..", "include", "moe_b200.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
-              "-shared", "-Xcompiler", "-fPIC"]
+              "-shared", "-Xcompiler", "-fPIC", "-t", "0"]     # -t 0: the sources side by side
 
 
 def _nvcc() -> str:

@@ -13,6 +13,8 @@
 // balance_join_kernel adds in chunk order (no floating-point atomics: the same bits every time).  Counts are integers.
 // Bound by latency (search of the borders, load, reductions) up to some thousand tokens and by the exponentials and
 // their reductions beyond; a row is loaded while the one before is worked on.
+// Measured, 256 experts, fp32: 16 tokens 4.7 us, 16384 tokens 17 us (two launches; 172 us when one CTA added 512 partial
+// rows in turn), 4099 tokens in 700 sequences of 160 experts 23 us; gradient of 8191 ragged bf16 tokens 9 us.
 #include "elem_device.cuh"
 
 namespace moe {

@@ -117,9 +117,13 @@ __device__ __forceinline__ float token_gate(const NormArgs& a, int64_t row) {
 // ---- Forward
 //
 // Bound by HBM (x, y in; s, h out), so the loads must never wait for the two reductions of a row: persistent CTAs bring
-// the rows of x, y (and a full gate) that they will need through a ring of up to three stages (cp.async).  Every thread copies
-// exactly the sixteen-byte pieces that it will read itself, so the ring needs no barrier.  Weights come from the first-level
-// cache, which the copies pass by.
+// the rows of x, y (and a full gate) that they will need through a ring of up to three stages (cp.async).  Every thread
+// copies exactly the sixteen-byte pieces that it will read itself, so the ring needs no barrier.  Weights come from the
+// first-level cache, which the copies pass by.  A thread has sixteen columns of a row of 4096 and more: two CTAs of 448
+// threads at 7168 columns, whose barriers fill each other's gaps.
+// Measured, 4096 x 7168 bf16: join and norm 47 us (5.0 TB/s), with e4m3 output 50 us (4.2 TB/s: 61 % of the issue slots
+// are taken, the conversion's maximum and products among them); without the ring 79 us.  4096 x 5001 (kEdges) 44 us, with
+// rows 5006 apart (kShifted) 59 us, element by element 180 us.
 constexpr int kMaxRing = 3;
 
 // Until the oldest of `ring` stages in flight has landed.
@@ -577,7 +581,9 @@ __global__ void __launch_bounds__(kNormThreads) block_norm_backward_kernel(NormA
 // ... and this one where parameters have the activations' type and a row fits 16 columns a thread and the ring: the
 // rows come through a ring like the forward's, the column sums stay in registers as fp32, and the weights, which leave no
 // registers for themselves, in shared memory behind the ring (an SM's quarter has 128 registers for each of four warps).
-// Missing parts are neutral values (y = 0, w_post = 1, gate = 1) instead of branches.
+// Missing parts are neutral values (y = 0, w_post = 1, gate = 1) instead of branches.  Bound by HBM at many rows (x, y, gh,
+// gs in; dx, dy out).  Measured, 16384 x 7168 bf16 with a gate per channel: 305 us (4.6 TB/s) for both kernels, 809 us with
+// the kernel above; 4096 x 7168 with a full gate 98 us (4.8 TB/s); 4096 x 5001 97 us.
 template <typename T, int CH, RowMode MODE, int GATE>
 __global__ void __launch_bounds__(kNormThreads) block_norm_backward_ring_kernel(NormArgs a) {
   griddep_launch_dependents();

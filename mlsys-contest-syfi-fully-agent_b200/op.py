@@ -291,6 +291,11 @@ def _aligned(t: Optional[torch.Tensor]) -> bool:
                          (t.dim() == 1 or t.shape[0] <= 1 or t.stride(0) * t.element_size() % 16 == 0))
 
 
+def _new_like(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape and type (``empty_like`` costs less, but keeps the layout of some views)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _on_gpu(t: torch.Tensor):
     if not t.is_cuda:
         raise ValueError("the tensors must be on a GPU: there is no CPU path")
@@ -363,14 +368,14 @@ def block_norm(x: torch.Tensor, pre_weight: torch.Tensor, y: Optional[torch.Tens
                 (args[6] == 2 or _aligned(gate))):
             raise ValueError("quantize needs rows that are 16-byte aligned")
     _on_gpu(x)
-    s = x if y is None else x.new_empty((T, H))
+    s = x if y is None else _new_like(x)
     rstd = x.new_empty((T, 2), dtype=torch.float32)
     scale = None
     if quantize:
         h = x.new_empty((T, H), dtype=torch.float8_e4m3fn)
         scale = x.new_empty((H // BLOCK, T), dtype=torch.float32)
     else:
-        h = x.new_empty((T, H))
+        h = _new_like(x)
     if T:
         _launch(loader.lib.moe_fp8_block_scale_block_norm, x.device, *args, eps, None if y is None else s.data_ptr(),
                 h.data_ptr(), scale.data_ptr() if quantize else None, rstd.data_ptr())
@@ -393,10 +398,10 @@ def block_norm_backward(x: torch.Tensor, pre_weight: torch.Tensor, rstd: torch.T
     gh, gh_stride = _rows("grad_h", grad_h, shape, dtype, dev)
     gs, gs_stride = (None, 0) if grad_stream is None else _rows("grad_stream", grad_stream, shape, dtype, dev)
     _on_gpu(x)
-    out = {"x": x.new_empty((T, H)), "pre_weight": torch.empty_like(pre_weight),
-           "y": None if y is None else x.new_empty((T, H)),
+    out = {"x": _new_like(x), "pre_weight": torch.empty_like(pre_weight),
+           "y": None if y is None else _new_like(x),
            "post_weight": None if post_weight is None else torch.empty_like(post_weight),
-           "gate": None if gate is None else gate.new_empty(gate.shape)}
+           "gate": None if gate is None else _new_like(gate)}
     if T == 0:                                     # the sums over no token
         for k in ("pre_weight", "post_weight", "gate"):
             if out[k] is not None:
