@@ -133,7 +133,7 @@ __device__ __forceinline__ void ring_wait(int ring) {
   else copies_wait<0>();
 }
 
-// The row's share of one thread in a stage: CH groups of eight columns of up to NARR arrays.
+// The row's share of one thread in a stage: CH groups of eight columns of every array.
 template <typename T, int CH>
 __device__ __forceinline__ uint32_t piece(int array, int c) {
   return (array * CH + c) * blockDim.x * sizeof(Pack8<T>) + threadIdx.x * 16;
@@ -217,22 +217,21 @@ __device__ __forceinline__ void put8(uint8_t* stage, int array, int c, const F2 
     *reinterpret_cast<uint4*>(stage + piece<T, CH>(array, c) + half * 16 * blockDim.x) = raw.w[half];
 }
 
-// Pieces behind the row's end are never copied: they hold zeros.
+// Pieces behind the end of an aligned row are never copied: they hold zeros.  (Rows with edges are clipped when they are read.)
 template <typename T, int CH>
-__device__ __forceinline__ void clear_ring_ends(uint8_t* ring, uint32_t stage_bytes, int stages, int arrays, int H, int off) {
+__device__ __forceinline__ void clear_ring_ends(uint8_t* ring, uint32_t stage_bytes, int stages, int arrays, int H) {
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    if (!partial(group_column(c, off), H)) continue;
+    if (group_column(c, 0) < H) continue;
     for (int i = 0; i < stages * arrays; ++i)
       for (int half = 0; half < static_cast<int>(sizeof(T)) / 2; ++half)
         *reinterpret_cast<uint4*>(ring + i / arrays * stage_bytes + piece<T, CH>(i % arrays, c) + half * 16 * blockDim.x) = make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
-// Rows that do not start on 16 bytes (an odd width or stride, a view) go through the ring as the aligned blocks that cover
-// them; the last one brings only the row's bytes, so that nothing behind the row is read, and the bytes in front of the
-// row lie in the same 16 bytes of the same allocation.  The columns a thread takes are then blockDim.x apart, not what it
-// copied itself: these kernels have a barrier after the wait.
+// Rows that start anywhere go through the ring as the aligned blocks that cover them; the last one brings only the row's
+// bytes, so that nothing behind the row is read, and the bytes in front of the row lie in the same 16 bytes of the same
+// allocation.  A thread then reads what others copied: these kernels have a barrier after the wait.
 __host__ __device__ constexpr int span_bytes(int H, int size) { return (H * size + 15) / 16 * 16 + 16; }
 
 template <typename T>
@@ -340,7 +339,7 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 3 : CH
       }
     }
   }
-  if (VEC) clear_ring_ends<T, CH>(ring, stage_bytes, a.ring, a.arrays, H, off);
+  if (MODE == kAligned) clear_ring_ends<T, CH>(ring, stage_bytes, a.ring, a.arrays, H);
   for (int i = 0; i < a.ring; ++i) fetch(smem_address(ring) + i * stage_bytes);
   T* s_out = static_cast<T*>(a.s) + blockIdx.x * static_cast<int64_t>(H);
   T* h_out = static_cast<T*>(a.h) + blockIdx.x * static_cast<int64_t>(H);
