@@ -256,7 +256,9 @@ int moe_fp8_block_scale_route_static(const float* routing_logits, const uint16_t
 /* ---- Operators around the shard: what a decoder layer does directly before the router and the experts and directly
  * after them.  No counterparts in the reference.  All are asynchronous on `stream`, can be captured in a CUDA graph,
  * keep nothing between calls, take device pointers and give the same bits for the same inputs.  Tensors carry a type
- * code; a stride is the distance of two rows in elements, the elements of a row are adjacent, outputs are contiguous. */
+ * code; a stride is the distance of two rows in elements, the elements of a row are adjacent, outputs are contiguous.
+ * At most 2^30 tokens and sequences.  Before a stream capture make one ordinary call of the same kind, so that its kernel
+ * is loaded.  MOE_B200_EINVAL for everything that is not described here. */
 #define MOE_B200_F32 0
 #define MOE_B200_BF16 1
 #define MOE_B200_F16 2
@@ -317,12 +319,12 @@ int moe_fp8_block_scale_balance_loss_backward(const float* grad_loss, const void
 
 /* Products of up to 256 (row, expert) pairs with 4-bit weights and group scales:
  *   out[p, n] = sum_k x[p / pairs_per_row, k] * (q[e, n, k] - z[e, n, k / G]) * scale[e, n, k / G],   e = experts[p]
- *   x [pairs / pairs_per_row, K], bf16 or fp16, rows 16-byte aligned; qweight u8 [E, N, K / 2]: two values a byte, the
- *   even k in the low half, 16-byte aligned; scale [E, N, K / G] in x's type or fp32 (scale_f32); zero u8 [E, N, K / G]
+ *   x [pairs / pairs_per_row, K], bf16 (|x| < 2^63) or fp16, rows 16-byte aligned; qweight u8 [E, N, K / 2], 16-byte aligned:
+ *   two values a byte, the even k in the low half; scale [E, N, K / G] in x's type or fp32 (scale_f32); zero u8 [E, N, K / G]
  *   with values 0..15, or NULL: 8; G 32, 64 or 128, K <= 2^20 a multiple of G; N <= 2^22
  *   experts i32 [pairs], E <= 1024: an expert outside [0, E) is not held here, its row of out is zero; NULL with E == 1 and
  *   pairs_per_row == 1: one matrix for all rows
- *   out [pairs, N] in x's type or fp32 (out_f32).  Sums are fp32; a weight's q - z is exact. */
+ *   out [pairs, N] in x's type or fp32 (out_f32).  Sums are fp32, formed as sum q x - z sum x per group. */
 int moe_fp8_block_scale_matvec_w4(const void* x, int64_t x_stride, int dtype, const uint8_t* qweight, const void* scale,
                                   int scale_f32, const uint8_t* zero, const int32_t* experts, int pairs,
                                   int pairs_per_row, int E, int N, int K, int G, void* out, int out_f32, void* stream);

@@ -449,7 +449,9 @@ extern "C" int moe_fp8_block_scale_balance_loss(const void* logits, int64_t logi
                                                 void* stream_v) {
   if (bad_common(T, E, K, S, dtype, scoring, cu_seqlens)) return MOE_B200_EINVAL;
   if (S == 0) return MOE_B200_OK;
-  if ((T > 0 && (!logits || !topk_idx)) || !loss || !counts || !tokens || !workspace || !aligned(workspace, 4))
+  if ((T > 0 && (!logits || !topk_idx)) || !loss || !counts || !tokens || !workspace || !aligned(workspace, 4) ||
+      !aligned(logits, element_size(dtype)) || !aligned(topk_idx, 4) || !aligned(cu_seqlens, 4) || !aligned(loss, 4) ||
+      !aligned(counts, 4) || !aligned(tokens, 4))
     return MOE_B200_EINVAL;
   if (workspace_bytes < moe_fp8_block_scale_balance_loss_workspace_bytes(T, E)) return MOE_B200_EWORKSPACE;
   BalanceArgs a = {};
@@ -476,7 +478,10 @@ extern "C" int moe_fp8_block_scale_balance_loss_backward(const float* grad_loss,
                                                          void* grad_logits, void* stream_v) {
   if (bad_common(T, E, K, S, dtype, scoring, cu_seqlens)) return MOE_B200_EINVAL;
   if (T == 0) return MOE_B200_OK;
-  if (!logits || !grad_logits || (S > 0 && (!grad_loss || !counts || !tokens))) return MOE_B200_EINVAL;
+  if (!logits || !grad_logits || (S > 0 && (!grad_loss || !counts || !tokens)) || !aligned(logits, element_size(dtype)) ||
+      !aligned(grad_logits, element_size(dtype)) || !aligned(cu_seqlens, 4) || !aligned(grad_loss, 4) || !aligned(counts, 4) ||
+      !aligned(tokens, 4))
+    return MOE_B200_EINVAL;
   BalanceArgs a = {};
   a.logits = logits; a.stride = logits_stride; a.cu = cu_seqlens; a.mask = token_mask;
   a.T = T; a.E = E; a.K = K; a.S = S; a.softmax = scoring == MOE_B200_SCORE_SOFTMAX;

@@ -541,7 +541,7 @@ extern "C" int moe_fp8_block_scale_matvec_w4(const void* x, int64_t x_stride, in
       (!experts && (E != 1 || pairs_per_row != 1)))
     return MOE_B200_EINVAL;
   if (pairs == 0) return MOE_B200_OK;
-  if (!x || !qweight || !scale || !out || !aligned(scale, scale_f32 ? 4 : 2) || !aligned(x, 16) || (pairs > pairs_per_row && x_stride % 8 != 0) || !aligned(qweight, 16))
+  if (!x || !qweight || !scale || !out || !aligned(scale, scale_f32 ? 4 : 2) || !aligned(out, out_f32 ? 4 : 2) || !aligned(experts, 4) || !aligned(x, 16) || (pairs > pairs_per_row && x_stride % 8 != 0) || !aligned(qweight, 16))
     return MOE_B200_EINVAL;
   MatvecArgs a = {x, x_stride, qweight, scale, zero, experts, pairs, pairs_per_row, E, N, K, scale_f32, out_f32, 1, 0, 0, out};
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);

@@ -148,7 +148,8 @@ def test_c_entry_points_refuse_before_touching_a_device(op, pkg):
     f = lib.moe_fp8_block_scale_balance_loss
     assert call(f, loss, _7=FAKE, _8=0) == F.OK
     for bad in (dict(_0=None), dict(_2=3), dict(_3=None), dict(_4=-1), dict(_5=0), dict(_5=1025), dict(_6=0), dict(_6=257),
-                dict(_8=2), dict(_8=-1), dict(_10=2), dict(_12=None), dict(_15=None), dict(_15=FAKE + 1)):
+                dict(_8=2), dict(_8=-1), dict(_10=2), dict(_12=None), dict(_15=None), dict(_15=FAKE + 1), dict(_0=FAKE + 2),
+                dict(_3=FAKE + 1), dict(_7=FAKE + 2), dict(_4=(1 << 30) + 1)):
         assert call(f, loss, **bad) == F.EINVAL, bad
     assert call(f, loss, _16=16) == F.EWORKSPACE
     back = [FAKE, FAKE, 256, F.F32, FAKE, FAKE, 4, 256, 8, None, 1, None, 0, 0.1, FAKE, None]
@@ -161,5 +162,5 @@ def test_c_entry_points_refuse_before_touching_a_device(op, pkg):
     assert call(f, mv, _8=0) == F.OK
     for bad in (dict(_0=None), dict(_0=FAKE + 2), dict(_1=255), dict(_2=F.F32), dict(_3=None), dict(_3=FAKE + 4),
                 dict(_4=None), dict(_8=257), dict(_8=-1), dict(_9=0), dict(_9=3), dict(_10=2), dict(_11=0), dict(_12=200),
-                dict(_13=16), dict(_14=None)):
+                dict(_13=16), dict(_14=None), dict(_14=FAKE + 1), dict(_4=FAKE + 1), dict(_7=FAKE + 2), dict(_11=(1 << 22) + 1)):
         assert call(f, mv, **bad) == F.EINVAL, bad
