@@ -263,6 +263,8 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
     }
   }
 
+  if (jobs.n == 0) return;                         // none of the batch's experts is held here: a batch of zero rows
+
   const int steps = (a.K + kStep - 1) / kStep, groups = a.K / G, tiles = (a.N + kTile - 1) / kTile;
   const int64_t items = static_cast<int64_t>(jobs.n) * tiles;
   // The CTA's run of items.  A run that goes on into the next job stages x twice and ends two rounds with idle warps, so

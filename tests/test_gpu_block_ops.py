@@ -488,6 +488,20 @@ def test_matvec_by_experts(op, g, T, k, E, N, K, G, t, zero, per_pair, span):
     assert not bool(out[outside].any())
 
 
+@pytest.mark.parametrize("T,k,per_pair", [(1, 8, False), (1, 1, True), (16, 8, False), (16, 8, True), (256, 1, True)])
+@pytest.mark.parametrize("far", [False, True])
+@pytest.mark.parametrize("ot", [None, F])
+def test_matvec_when_no_expert_is_held(op, g, T, k, per_pair, far, ot):
+    """A batch whose choices all lie on other shards, in front of this one's experts and behind them: zeros everywhere."""
+    E, N, K = 4, 100, 512
+    x, q, scale, z = matvec_inputs(g, T * k if per_pair else T, N, K, 64, BF, E, True)
+    e = torch.randint(E, 2 ** 31 - 1 if far else E + 3, (T, k), generator=g, device="cuda", dtype=torch.int32)
+    e = torch.where(torch.rand((T, k), generator=g, device="cuda") < 0.5, e, E - 1 - e).contiguous()
+    assert not bool(((e >= 0) & (e < E)).any())
+    out = op.matvec_w4(x, q, scale, z, experts=e.view(-1) if per_pair else e, out_dtype=ot)
+    assert out.shape == ((T * k, N) if per_pair else (T, k, N)) and not bool(out.any())
+
+
 def test_matvec_of_no_rows(op, g):
     x, q, scale, _ = matvec_inputs(g, 0, 5, 64, 32, BF)
     assert op.matvec_w4(x, q, scale).shape == (0, 5)
