@@ -281,7 +281,7 @@ extern "C" int moe_fp8_block_scale_block_norm(const void* x, int64_t x_stride, c
   }
   if (bad_common(a, dtype, param_f32) || !(eps > 0.0f)) return MOE_B200_EINVAL;
   if (T == 0) return MOE_B200_OK;
-  if (!x || !pre_weight || !h || !rstd || !aligned(rstd, 8) || (y && !stream_out)) return MOE_B200_EINVAL;
+  if (!x || !pre_weight || !h || !rstd || !aligned(rstd, 8) || !aligned(h_scale, 4) || (y && !stream_out)) return MOE_B200_EINVAL;
   const RowMode mode = row_mode(a, dtype);
   if (h_scale && (H % kBlock != 0 || mode != kAligned)) return MOE_B200_EINVAL;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);

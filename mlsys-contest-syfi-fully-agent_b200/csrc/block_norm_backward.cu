@@ -444,6 +444,10 @@ extern "C" int moe_fp8_block_scale_block_norm_backward(
   if (!x || !pre_weight || !rstd || !aligned(rstd, 8) || !grad_h || !grad_x || !grad_pre_weight || (y && !grad_y) ||
       (post_weight && !grad_post_weight) || (gate_kind != kGateNone && !grad_gate) || !workspace || !aligned(workspace, 16))
     return MOE_B200_EINVAL;
+  const int size = element_size(dtype);
+  if (!aligned(grad_pre_weight, a.pre_f32 ? 4 : size) || !aligned(grad_post_weight, a.post_f32 ? 4 : size) ||
+      !aligned(grad_gate, a.gate_f32 ? 4 : size))
+    return MOE_B200_EINVAL;
   if (workspace_bytes < moe_fp8_block_scale_block_norm_backward_workspace_bytes(T, H)) return MOE_B200_EWORKSPACE;
   ColumnSumArgs cs = {};
   a.sum_post = a.sum_gate = -1;

@@ -164,3 +164,20 @@ def test_c_entry_points_refuse_before_touching_a_device(op, pkg):
                 dict(_4=None), dict(_8=257), dict(_8=-1), dict(_9=0), dict(_9=3), dict(_10=2), dict(_11=0), dict(_12=200),
                 dict(_13=16), dict(_14=None), dict(_14=FAKE + 1), dict(_4=FAKE + 1), dict(_7=FAKE + 2), dict(_11=(1 << 22) + 1)):
         assert call(f, mv, **bad) == F.EINVAL, bad
+
+
+def test_c_entry_points_refuse_results_that_are_not_aligned_to_their_elements(op, pkg):
+    """A pointer between two elements would be a misaligned store on the device."""
+    lib, F = pkg.loader.lib, pkg.loader
+    for dtype, param_f32, element in ((F.F32, 0, 4), (F.BF16, 0, 2), (F.F16, 7, 4)):
+        for off in range(1, element):
+            def backward(kind, grads):
+                return lib.moe_fp8_block_scale_block_norm_backward(
+                    FAKE, 256, FAKE, 256, FAKE, 256, kind, FAKE, FAKE, 4, 256, dtype, param_f32, 1.0, FAKE, FAKE, 256, None, 0,
+                    FAKE, FAKE, *[FAKE + off if k == grads else FAKE for k in ("gate", "pre", "post")], FAKE, 1 << 40, None)
+            for kind in (1, 2, 3):
+                for grads in ("gate", "pre", "post"):
+                    assert backward(kind, grads) == F.EINVAL, (dtype, off, kind, grads)
+    for off in (1, 2, 3):
+        assert lib.moe_fp8_block_scale_block_norm(FAKE, 256, None, 0, None, 0, 0, FAKE, None, 4, 256, F.BF16, 0, 1.0, 1e-6,
+                                                  None, FAKE, FAKE + off, FAKE, None) == F.EINVAL, off
