@@ -265,12 +265,15 @@ def _launch(fn, dev: torch.device, *args):
     """Calls an entry point of the library with ``dev`` current and its stream as the last argument.  (A decode step's
     kernel takes a few microseconds: the calls below spend as little host time as they can, so checks are written
     without helpers that would format a message that is not needed.)"""
-    index = dev.index
-    if index == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    try:
+        current = torch._C._cuda_getDevice()
+    except AttributeError:      # a torch build without the raw getter
+        current = torch.cuda.current_device()
+    if dev.index == current:
+        rc = fn(*args, _stream_of(dev))
     else:
-        with torch.cuda.device(index):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        with torch.cuda.device(dev.index):
+            rc = fn(*args, _stream_of(dev))
     if rc:
         loader.check(rc)
 

@@ -181,3 +181,43 @@ def test_c_entry_points_refuse_results_that_are_not_aligned_to_their_elements(op
     for off in (1, 2, 3):
         assert lib.moe_fp8_block_scale_block_norm(FAKE, 256, None, 0, None, 0, 0, FAKE, None, 4, 256, F.BF16, 0, 1.0, 1e-6,
                                                   None, FAKE, FAKE + off, FAKE, None) == F.EINVAL, off
+
+
+@pytest.mark.parametrize("getters", [True, False])
+@pytest.mark.parametrize("current", [0, 1])
+def test_launches_on_the_tensors_device_with_its_stream(op, monkeypatch, getters, current):
+    """Also where another device is current, and with a torch build that lacks the raw getters; on stand-ins for the
+    device's state."""
+    state = {"device": current}
+
+    class device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, state["device"] = state["device"], self.index
+
+        def __exit__(self, *exc):
+            state["device"] = self.before
+
+    class Stream:
+        def __init__(self, dev):
+            self.cuda_stream = 100 + (dev if isinstance(dev, int) else dev.index)
+
+    for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"):
+        monkeypatch.delattr(torch._C, name, raising=False)
+    if getters:
+        monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: state["device"], raising=False)
+        monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 100 + index, raising=False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: state["device"])
+    monkeypatch.setattr(torch.cuda, "current_stream", Stream)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    seen = []
+
+    def entry(*args):
+        seen.append((state["device"], args))
+        return 0
+    op._launch(entry, torch.device("cuda", 1), 7, 8)
+    assert seen == [(1, (7, 8, 101))] and state["device"] == current
+    with pytest.raises(op.loader.MoeLibraryError):
+        op._launch(lambda *args: op.loader.EINVAL, torch.device("cuda", 1))
