@@ -19,8 +19,11 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmoe_b200.so")
 LIB_TVMFFI = os.path.join(HERE, "libmoe_b200_tvmffi.so")
 
-SOURCES = ["launcher.cu", "route_permute.cu", "grouped_gemm.cu", "grouped_gemm_large.cu", "decode_kernel.cu", "swiglu_combine.cu", "static_entry.cu", "quantize.cu", "ep_push.cu", "block_norm.cu", "block_norm_backward.cu", "balance_loss.cu", "matvec_w4.cu"]
-HEADERS = ["kernels.h", "moe_layout.h", "ptx.cuh", "route_device.cuh", "epilogue_device.cuh", "gemm_common.cuh", "map_cache.h", "elem_device.cuh", "block_norm.cuh", os.path.join("..", "..", "include", "moe_b200.h")]
+SOURCES = ["launcher.cu", "route_permute.cu", "grouped_gemm.cu", "grouped_gemm_large.cu", "decode_kernel.cu", "swiglu_combine.cu", "static_entry.cu", "quantize.cu", "ep_push.cu"]
+HEADERS = ["kernels.h", "moe_layout.h", "ptx.cuh", "route_device.cuh", "epilogue_device.cuh", "gemm_common.cuh", "map_cache.h", os.path.join("..", "..", "include", "moe_b200.h")]
+# The operators around the shard: in the C-ABI library, not in what a harness compiles for `run`
+SOURCES_AROUND = ["block_norm.cu", "block_norm_backward.cu", "balance_loss.cu", "matvec_w4.cu"]
+HEADERS_AROUND = ["elem_device.cuh", "block_norm.cuh"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
               "-shared", "-Xcompiler", "-fPIC", "-t", "0"]     # -t 0: the sources side by side
 
@@ -52,19 +55,19 @@ def _compile(sources, out_dir: str, flags=()):
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Both libraries from one set of object files."""
-    srcs = [os.path.join(CSRC, s) for s in SOURCES]
-    deps = srcs + [os.path.join(CSRC, h) for h in HEADERS] + [os.path.abspath(__file__)]
+    """Both libraries; the sources that they share are compiled once."""
+    shard, around = ([os.path.join(CSRC, s) for s in names] for names in (SOURCES, SOURCES_AROUND))
+    deps = shard + [os.path.join(CSRC, h) for h in HEADERS] + [os.path.abspath(__file__)]
     shim = os.path.join(CSRC, "tvm_ffi_shim.cu")
-    lib = force or _stale(LIB, deps)
+    lib = force or _stale(LIB, deps + around + [os.path.join(CSRC, h) for h in HEADERS_AROUND])
     ffi = tvmffi_paths() is not None and os.path.exists(shim) and (force or _stale(LIB_TVMFFI, deps + [shim]))
     if lib or ffi:
         with tempfile.TemporaryDirectory() as tmp:
-            objects = _compile(srcs, tmp, ["-Xptxas", "-v"] if verbose else [])
+            objects = _compile(shard + (around if lib else []), tmp, ["-Xptxas", "-v"] if verbose else [])
             if lib:
                 subprocess.run([_nvcc()] + NVCC_FLAGS + ["-o", LIB] + objects, check=True, cwd=CSRC)
             if ffi:
-                build_tvmffi(force=True, objects=objects)
+                build_tvmffi(force=True, objects=objects[:len(shard)])
     return LIB
 
 
@@ -81,7 +84,7 @@ def tvmffi_paths():
 
 
 def build_tvmffi(force: bool = False, objects=None):
-    """The harness-facing shim: same sources (or their object files) plus csrc/tvm_ffi_shim.cu."""
+    """The harness-facing shim: the shard's sources (or their object files) plus csrc/tvm_ffi_shim.cu."""
     shim = os.path.join(CSRC, "tvm_ffi_shim.cu")
     paths = tvmffi_paths()
     if paths is None or not os.path.exists(shim):

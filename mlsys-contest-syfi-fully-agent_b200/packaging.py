@@ -23,7 +23,7 @@ DEFINITION = "moe_fp8_block_scale_ds_routing_topk8_ng8_kg4_e32_h7168_i2048"
 AUTHOR = "b200-native"
 ENTRY_POINT = "tvm_ffi_shim.cu::run"
 
-# everything the library is built from, the tvm-ffi shim first
+# everything that `run` is built from, the tvm-ffi shim first
 SOURCE_FILES = ["tvm_ffi_shim.cu"] + build.SOURCES + [h for h in build.HEADERS if not h.startswith("..")]
 
 

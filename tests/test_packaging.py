@@ -49,3 +49,20 @@ def test_every_source_of_the_library_is_packed(pkg):
     """A missing source still links as a shared library and fails only when the harness loads it."""
     assert set(pkg.build.SOURCES) <= set(pkg.packaging.SOURCE_FILES)
     assert {h for h in pkg.build.HEADERS if not h.startswith("..")} <= set(pkg.packaging.SOURCE_FILES)
+
+
+def test_only_what_the_entry_point_reaches_is_packed(pkg):
+    """The harness compiles the packed files one after another and calls nothing but ``run``: the operators around the shard
+    are in the C-ABI library alone."""
+    b = pkg.build
+    around = set(b.SOURCES_AROUND) | set(b.HEADERS_AROUND)
+    assert {"block_norm.cu", "block_norm_backward.cu", "balance_loss.cu", "matvec_w4.cu"} <= around
+    assert not around & set(pkg.packaging.SOURCE_FILES) and not set(b.SOURCES_AROUND) & set(b.SOURCES)
+    files = set(os.listdir(b.CSRC))
+    assert files == set(b.SOURCES) | {h for h in b.HEADERS if not h.startswith("..")} | around | {"tvm_ffi_shim.cu"}
+    b.build()
+    exports = lambda lib: subprocess.run(["nm", "-D", "--defined-only", lib], check=True, capture_output=True, text=True).stdout  # noqa: E731
+    names = [n for n in pkg.loader.EXPORTS if any(k in n for k in ("block_norm", "balance_loss", "matvec"))]
+    assert len(names) == 7 and all(n in exports(b.LIB) for n in names)
+    if b.tvmffi_paths() is not None:
+        assert not any(n in exports(b.LIB_TVMFFI) for n in names)
