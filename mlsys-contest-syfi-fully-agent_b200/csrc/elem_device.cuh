@@ -138,6 +138,16 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// sum += v, and what the sum's last bit cannot hold goes to `lost` (the error of an addition, after Knuth).  Only for sums of
+// sums: the chain of additions is as long as without it.
+__device__ __forceinline__ void add_exactly(float& sum, float& lost, float v) {
+  const float s = sum + v, b = s - sum;
+  lost += (sum - (s - b)) + (v - b);
+  sum = s;
+}
+// The two joined; an infinite or undefined sum has nothing to add.
+__device__ __forceinline__ float joined(float sum, float lost) { return isfinite(lost) ? sum + lost : sum; }
+
 // Sums of N values over the CTA, the same bits in every thread.  `red` holds N * 32 floats that no other reduction in
 // flight uses: one barrier per call, so consecutive calls alternate between two areas.
 template <int N>

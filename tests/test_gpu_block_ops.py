@@ -634,3 +634,40 @@ def test_rows_far_into_a_long_batch(op, g):
     r, size = norm_grad_ref(h[-2:], None, rstd[-2:], x[-2:], w)["x"]
     near(dx[-2:], r, size)
     assert not bool(dx[1000:1010].any())
+
+
+# ---------------------------------------------------------------------------- sums over long batches
+
+
+@pytest.mark.parametrize("T,H,t,gate,f32", [
+    (2 ** 23 + 77, 8, F, "channel", False),       # the ring kernel, thousands of rows per CTA
+    (2 ** 22 + 5, 9, F, "channel", False),        # with edges
+    (2 ** 22 + 5, 8, BF, "channel", True),        # the other kernel, rows of 16 bytes
+    (2 ** 22, 7, HF, "none", True),               # and element by element
+    (148 * 256 + 1, 4608, F, "none", False),      # one row more than a wave of CTAs takes
+])
+def test_weight_gradients_of_a_long_batch(op, g, T, H, t, gate, f32):
+    """Equal rows, so that all terms of a column have one sign and every addition rounds the same way.  A CTA adds at most
+    256 terms in a row, an error of 256 * 2^-24 / 2 of the sum; what comes after keeps its errors; the terms themselves
+    have fewer than 20 roundings: 148 * 2^-24 together, below 2 * 2^-17."""
+    row = norm_inputs(g, 1, H, t, gate, f32=f32)
+    rows = lambda v: v.expand(T, H).contiguous()  # noqa: E731
+    rstd = torch.tensor([[1.37, 0.83]], device="cuda")
+    gh, gs = (torch.randn((1, H), generator=g, device="cuda").to(t) for _ in range(2))
+    ref = norm_grad_ref(gh, gs, rstd, *ref_args(row))
+    got = op.block_norm_backward(rstd=rstd.expand(T, 2).contiguous(), grad_h=rows(gh), grad_stream=rows(gs),
+                                 **dict(row, x=rows(row["x"]), y=rows(row["y"])))
+    for k in ("pre_weight", "post_weight", "gate"):
+        if got[k] is not None:
+            near(got[k], ref[k][0] * T, ref[k][1] * T, 2.0 ** -17)
+    near(got["x"][-1:], *ref["x"])
+
+
+def test_weight_gradients_of_infinite_terms(op):
+    """An infinite sum stays infinite, a NaN stays in its column."""
+    x = torch.ones((40_000, 16), device="cuda")
+    gh = torch.ones_like(x)
+    gh[5, 1], gh[7, 2], gh[39_999, 3] = float("inf"), float("nan"), float("-inf")
+    rstd = torch.ones((40_000, 2), device="cuda")
+    dw = op.block_norm_backward(x, torch.ones(16, device="cuda"), rstd, gh)["pre_weight"].tolist()
+    assert dw[1] == float("inf") and dw[2] != dw[2] and dw[3] == float("-inf") and dw[4:] == [40_000.0] * 12
