@@ -671,3 +671,19 @@ def test_weight_gradients_of_infinite_terms(op):
     rstd = torch.ones((40_000, 2), device="cuda")
     dw = op.block_norm_backward(x, torch.ones(16, device="cuda"), rstd, gh)["pre_weight"].tolist()
     assert dw[1] == float("inf") and dw[2] != dw[2] and dw[3] == float("-inf") and dw[4:] == [40_000.0] * 12
+
+
+@pytest.mark.parametrize("T,E,K,cu", [(2 ** 23 + 3, 2, 1, None), (2 ** 23 + 3, 2, 2, [5, 3_000_001, 8_000_000]), (700_001, 600, 6, None)])
+def test_balance_loss_of_a_long_batch(op, g, T, E, K, cu):
+    """Equal rows of logits, as above.  256 additions a warp, 32 for a CTA's warps, 148 for rows of chunks: 218 * 2^-24 of the sum
+    at most, and a few roundings of the terms: below 2 * 2^-17."""
+    _, idx, borders, _ = balance_inputs(g, T, E, K, F, cu)
+    logits = torch.randn((1, E), generator=g, device="cuda").expand(T, E).contiguous()
+    loss, counts, tokens = op.balance_loss(logits, idx, 0.3, cu_seqlens=borders)
+    p = torch.sigmoid(logits[0].to(D))
+    p = p / p.sum()
+    for q, (lo, hi) in enumerate(zip((cu or [0, T])[:-1], (cu or [0, T])[1:])):
+        c = torch.bincount(idx[lo:hi].flatten().long(), minlength=E)
+        assert torch.equal(counts[q].long(), c) and int(tokens[q]) == hi - lo
+        ref = 0.3 * E / K * (c.to(D) * p).sum() / (hi - lo)
+        near(loss[q], ref, ref, 2.0 ** -17)
