@@ -319,12 +319,13 @@ int moe_fp8_block_scale_balance_loss_backward(const float* grad_loss, const void
 
 /* Products of up to 256 (row, expert) pairs with 4-bit weights and group scales:
  *   out[p, n] = sum_k x[p / pairs_per_row, k] * (q[e, n, k] - z[e, n, k / G]) * scale[e, n, k / G],   e = experts[p]
- *   x [pairs / pairs_per_row, K], bf16 (|x| < 2^63) or fp16, rows 16-byte aligned; qweight u8 [E, N, K / 2], 16-byte aligned:
+ *   x [pairs / pairs_per_row, K], bf16 or fp16, rows 16-byte aligned; qweight u8 [E, N, K / 2], 16-byte aligned:
  *   two values a byte, the even k in the low half; scale [E, N, K / G] in x's type or fp32 (scale_f32); zero u8 [E, N, K / G]
  *   with values 0..15, or NULL: 8; G 32, 64 or 128, K <= 2^20 a multiple of G; N <= 2^22
  *   experts i32 [pairs], E <= 1024: an expert outside [0, E) is not held here, its row of out is zero; NULL with E == 1 and
  *   pairs_per_row == 1: one matrix for all rows
- *   out [pairs, N] in x's type or fp32 (out_f32).  Sums are fp32, formed as sum q x - z sum x per group. */
+ *   out [pairs, N] in x's type or fp32 (out_f32).  Sums are fp32.  With out_f32 q - z is formed exactly; for a 16-bit result a
+ *   group's sum is sum q x - z sum x, whose error goes with sum |q x|, and bf16 wants |x| < 2^63. */
 int moe_fp8_block_scale_matvec_w4(const void* x, int64_t x_stride, int dtype, const uint8_t* qweight, const void* scale,
                                   int scale_f32, const uint8_t* zero, const int32_t* experts, int pairs,
                                   int pairs_per_row, int E, int N, int K, int G, void* out, int out_f32, void* stream);

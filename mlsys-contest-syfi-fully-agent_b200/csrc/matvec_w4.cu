@@ -10,12 +10,18 @@
 // 32) weights feed eight (four, two) products in whatever order of k suits the unpacking; x is staged in shared memory in
 // that same order.
 //
-// Unpacking is one AND per pair: a floating-point format's codes are linear up to twice its smallest normal number, so a
-// half word with only a 4-bit field set is q or 16 q times the smallest subnormal (2^-24 in fp16, 2^-133 in bf16), which
-// the tensor cores multiply exactly.  The fields at bit 0 and at bit 4 go to accumulators of their own.  bf16 activations
-// are staged times 2^64 so that the products are normal fp32 numbers (|x| < 2^63; below 2^-57 they keep an absolute 2^-80).
-// Products and sums are fp32; per group:  sum (q - z) x = sum q x - z sum x, with sum x from the staging, and the scale
-// multiplies the fp32 result.
+// Unpacking begins with one AND per pair: a floating-point format's codes are linear up to twice its smallest normal number,
+// so a half word with only a 4-bit field set is q or 16 q times the smallest subnormal (2^-24 in fp16, 2^-133 in bf16).  The
+// fields at bit 0 and at bit 4 go to accumulators of their own.  Products and sums are fp32; the scale multiplies a group's
+// fp32 sum.  What happens to the zero point depends on the result's type:
+// * fp32 results (EXACT): one packed multiply-add per pair,  code * 2^127 - z 2^-6  (bf16; 2^15 and 2^-9 in fp16), makes it
+//   (q - z) times a power of two, exactly, so the error goes with sum |(q - z) x| however close to the zero point the weights
+//   are.
+// * 16-bit results: the tensor cores multiply the codes themselves, exactly, and per group  sum (q - z) x = sum q x - z sum x,
+//   with sum x from the staging.  The error goes with sum |q x|, 2^-24 of it in each addition, which the result's own
+//   rounding of 2^-9 or 2^-12 hides.  bf16 activations are staged times 2^64 so that the products are normal fp32 numbers
+//   (|x| < 2^63; below 2^-57 they keep an absolute 2^-80).  The multiply-adds would cost one token through eight 4096 x 7168
+//   experts 35.1 us instead of 31.9, and sixteen tokens through 32 of them 120 instead of 108.
 //
 // One persistent CTA per SM takes a contiguous run of items (expert and up to 8 or 16 of its rows, 16 weight rows), stages
 // the rows of x that the expert has, and its sixteen warps stream weights through rings of their own (cp.async, two
@@ -59,6 +65,13 @@ struct MatvecArgs {
 template <typename T> struct Mma;
 template <> struct Mma<__nv_bfloat16> {
   static constexpr float kUnit = 0x1p69f;              // undoes 2^-133 of the codes and 2^64 of x
+  static constexpr float kExactUnit = 0x1p6f;          // undoes 2^-6 of q - z
+  static constexpr uint32_t kEven = 0x7F007F00u, kOdd = 0x7D007D00u, kMinus = 0xFF00FF00u, kEight = 0xBE00BE00u;   // 2^127, 2^123, -2^127, -8 2^-6
+  static __device__ __forceinline__ uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+  }
   static __device__ __forceinline__ uint32_t staged(uint32_t v) {
     const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v), __floats2bfloat162_rn(0x1p64f, 0x1p64f));
     return *reinterpret_cast<const uint32_t*>(&r);
@@ -72,6 +85,13 @@ template <> struct Mma<__nv_bfloat16> {
 };
 template <> struct Mma<__half> {
   static constexpr float kUnit = 0x1p24f;
+  static constexpr float kExactUnit = 0x1p9f;
+  static constexpr uint32_t kEven = 0x78007800u, kOdd = 0x68006800u, kMinus = 0xF800F800u, kEight = 0xA400A400u;   // 2^15, 2^11, -2^15, -8 2^-9
+  static __device__ __forceinline__ uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+  }
   static __device__ __forceinline__ uint32_t staged(uint32_t v) { return v; }
   static __device__ __forceinline__ float2 widen(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
   static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
@@ -156,15 +176,15 @@ __device__ __forceinline__ void find_jobs(const MatvecArgs& a, int max_cols, Job
   __syncthreads();
 }
 
-template <typename T>
+template <typename T, bool EXACT>
 __device__ __forceinline__ void store_result(const MatvecArgs& a, int pair, int n, float v) {
   const int64_t at = static_cast<int64_t>(pair) * a.N + n;
-  if (a.out_f32) static_cast<float*>(a.out)[at] = v;
+  if (EXACT) static_cast<float*>(a.out)[at] = v;
   else static_cast<T*>(a.out)[at] = from_f32<T>(v);
 }
 
-// sum += the products of a stage, 16 rows and 256 columns with USED of NT column tiles, times 1 / kUnit.
-template <typename T, int G, int USED, int NT, bool ZERO>
+// sum += the products of a stage, 16 rows and 256 columns with USED of NT column tiles, times 1 / kUnit (kExactUnit).
+template <typename T, int G, int USED, int NT, bool ZERO, bool EXACT>
 __device__ __forceinline__ void step(const MatvecArgs& a, const uint8_t* stage, const uint8_t* const (&x_at)[NT], const float* xs_at,
                                      int u, const int (&s_at)[2], const int (&z_low)[2], int gid, int quad, float (&sum)[NT][4]) {
   using S = Stage<G, ZERO>;
@@ -196,13 +216,29 @@ __device__ __forceinline__ void step(const MatvecArgs& a, const uint8_t* stage, 
       const int r = gid + 8 * h, byte = gi * (G / 2) + quad * (4 * W);
       w[h] = *reinterpret_cast<const typename Words<W>::Type*>(stage + r * (kStep / 2) + ((byte >> 4) ^ swizzle(r)) * 16 + (byte & 15));
     }
+    uint32_t minus[2];                             // EXACT: -z of the lane's two rows, in the operands' unit
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      minus[h] = Mma<T>::kEight;
+      if (ZERO && EXACT) {
+        const uint32_t z = stage[S::kZeros + (gid + 8 * h) * 4 * S::kZeroWords + ((z_low[h] + u * S::kGroups) & 3) + gi];
+        minus[h] = Mma<T>::fma(z | z << 16, Mma<T>::kMinus, 0u);
+      }
+    }
     float even[USED][4] = {}, odd[USED][4] = {};   // sums over the fields at bit 0 and at bit 4 of a byte
 #pragma unroll
     for (int j = 0; j < W; ++j) {
       const uint32_t lo = reinterpret_cast<const uint32_t*>(&w[0])[j];
       const uint32_t hi = reinterpret_cast<const uint32_t*>(&w[1])[j];
-      const uint32_t fe[4] = {lo & 0x000F000Fu, hi & 0x000F000Fu, (lo >> 8) & 0x000F000Fu, (hi >> 8) & 0x000F000Fu};
-      const uint32_t fo[4] = {lo & 0x00F000F0u, hi & 0x00F000F0u, (lo >> 8) & 0x00F000F0u, (hi >> 8) & 0x00F000F0u};
+      uint32_t fe[4] = {lo & 0x000F000Fu, hi & 0x000F000Fu, (lo >> 8) & 0x000F000Fu, (hi >> 8) & 0x000F000Fu};
+      uint32_t fo[4] = {lo & 0x00F000F0u, hi & 0x00F000F0u, (lo >> 8) & 0x00F000F0u, (hi >> 8) & 0x00F000F0u};
+      if (EXACT) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          fe[i] = Mma<T>::fma(fe[i], Mma<T>::kEven, minus[i & 1]);
+          fo[i] = Mma<T>::fma(fo[i], Mma<T>::kOdd, minus[i & 1]);
+        }
+      }
 #pragma unroll
       for (int t = 0; t < USED; ++t) {
         const uint4 b = *reinterpret_cast<const uint4*>(x_at[t] + gi * (2 * G) + 64 * j);
@@ -210,18 +246,25 @@ __device__ __forceinline__ void step(const MatvecArgs& a, const uint8_t* stage, 
         Mma<T>::run(odd[t], fo, b.z, b.w, odd[t]);
       }
     }
-    float2 xt[USED];
+    if constexpr (EXACT) {
 #pragma unroll
-    for (int t = 0; t < USED; ++t) xt[t] = *reinterpret_cast<const float2*>(xs_at + gi * (8 * NT) + 8 * t);
+      for (int t = 0; t < USED; ++t)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = gid + 8 * h;
-      float zero = 8.0f;
-      if (ZERO) zero = static_cast<float>(stage[S::kZeros + r * 4 * S::kZeroWords + ((z_low[h] + u * S::kGroups) & 3) + gi]);
+        for (int i = 0; i < 4; ++i) sum[t][i] += (even[t][i] + odd[t][i]) * scale[gi][i >> 1];
+    } else {
+      float2 xt[USED];
 #pragma unroll
-      for (int t = 0; t < USED; ++t) {
-        sum[t][2 * h] += (even[t][2 * h] + 0.0625f * odd[t][2 * h] - zero * xt[t].x) * scale[gi][h];
-        sum[t][2 * h + 1] += (even[t][2 * h + 1] + 0.0625f * odd[t][2 * h + 1] - zero * xt[t].y) * scale[gi][h];
+      for (int t = 0; t < USED; ++t) xt[t] = *reinterpret_cast<const float2*>(xs_at + gi * (8 * NT) + 8 * t);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = gid + 8 * h;
+        float zero = 8.0f;
+        if (ZERO) zero = static_cast<float>(stage[S::kZeros + r * 4 * S::kZeroWords + ((z_low[h] + u * S::kGroups) & 3) + gi]);
+#pragma unroll
+        for (int t = 0; t < USED; ++t) {
+          sum[t][2 * h] += (even[t][2 * h] + 0.0625f * odd[t][2 * h] - zero * xt[t].x) * scale[gi][h];
+          sum[t][2 * h + 1] += (even[t][2 * h + 1] + 0.0625f * odd[t][2 * h + 1] - zero * xt[t].y) * scale[gi][h];
+        }
       }
     }
   }
@@ -235,12 +278,12 @@ struct Cursor {
   int slice_steps, slices;   // of x
 };
 
-// G: group size.  NT: token tiles of eight columns.  ZERO: a table of zero points.
-template <typename T, int G, int NT, bool ZERO>
+// G: group size.  NT: token tiles of eight columns.  ZERO: a table of zero points.  EXACT: fp32 results.
+template <typename T, int G, int NT, bool ZERO, bool EXACT>
 __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
   using S = Stage<G, ZERO>;
   constexpr int W = G / 32, kCols = 8 * NT;
-  extern __shared__ __align__(16) uint8_t smem[];  // rings of the warps, staged x, a group of zeros, sums of x
+  extern __shared__ __align__(16) uint8_t smem[];  // rings of the warps, staged x, a group of zeros, sums of x (!EXACT)
   __shared__ float red[2][kWarps][kCols][kTile + 4];
   __shared__ Jobs jobs;
   __shared__ int scan[kWarps];
@@ -259,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
   for (int w = 0; w < kMaxPairs / 32; ++w) {
     for (uint32_t left = jobs.missing[w]; left != 0; left &= left - 1) {
       const int p = w * 32 + __ffs(left) - 1;
-      for (int n = blockIdx.x * kThreads + tid; n < a.N; n += gridDim.x * kThreads) store_result<T>(a, p, n, 0.0f);
+      for (int n = blockIdx.x * kThreads + tid; n < a.N; n += gridDim.x * kThreads) store_result<T, EXACT>(a, p, n, 0.0f);
     }
   }
 
@@ -403,14 +446,18 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
             for (int c = 0; c < cols; ++c) {
               uint4 v = make_uint4(0u, 0u, 0u, 0u);
               if (i < held) v = __ldg(reinterpret_cast<const uint4*>(x_from[c]) + i);
-              xs[c * x_row + to] =
-                  make_uint4(Mma<T>::staged(__byte_perm(v.x, v.z, 0x5410)), Mma<T>::staged(__byte_perm(v.y, v.w, 0x5410)),
-                             Mma<T>::staged(__byte_perm(v.x, v.z, 0x7632)), Mma<T>::staged(__byte_perm(v.y, v.w, 0x7632)));
-              const float2 p = Mma<T>::widen(v.x), q = Mma<T>::widen(v.y), r = Mma<T>::widen(v.z), t = Mma<T>::widen(v.w);
-              float total = ((p.x + p.y) + (q.x + q.y)) + ((r.x + r.y) + (t.x + t.y));
+              const uint4 pairs = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.y, v.w, 0x5410),
+                                             __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x7632));
+              if constexpr (EXACT) {
+                xs[c * x_row + to] = pairs;
+              } else {
+                xs[c * x_row + to] = make_uint4(Mma<T>::staged(pairs.x), Mma<T>::staged(pairs.y), Mma<T>::staged(pairs.z), Mma<T>::staged(pairs.w));
+                const float2 p = Mma<T>::widen(v.x), q = Mma<T>::widen(v.y), r = Mma<T>::widen(v.z), t = Mma<T>::widen(v.w);
+                float total = ((p.x + p.y) + (q.x + q.y)) + ((r.x + r.y) + (t.x + t.y));
 #pragma unroll
-              for (int d = G / 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
-              if (in == 0) xsum[i / (G / 8) * kCols + c] = total * (1.0f / Mma<T>::kUnit);
+                for (int d = G / 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
+                if (in == 0) xsum[i / (G / 8) * kCols + c] = total * (1.0f / Mma<T>::kUnit);
+              }
             }
           }
           __syncthreads();
@@ -440,8 +487,8 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
           copies_wait<kDepth - 1>();
           __syncwarp();
           const float* const xs_at = xsum + (at.u - s0) * (S::kGroups * kCols) + 2 * quad;
-          if (NT == 1 || cols <= 8) step<T, G, 1, NT, ZERO>(a, stage, x_at, xs_at, at.u, s_at, z_low, gid, quad, sum);
-          else step<T, G, NT, NT, ZERO>(a, stage, x_at, xs_at, at.u, s_at, z_low, gid, quad, sum);
+          if (NT == 1 || cols <= 8) step<T, G, 1, NT, ZERO, EXACT>(a, stage, x_at, xs_at, at.u, s_at, z_low, gid, quad, sum);
+          else step<T, G, NT, NT, ZERO, EXACT>(a, stage, x_at, xs_at, at.u, s_at, z_low, gid, quad, sum);
 #pragma unroll
           for (int t = 0; t < NT; ++t) x_at[t] += x_step[t];
           __syncwarp();
@@ -453,14 +500,14 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sum[t][k] *= Mma<T>::kUnit;
+        for (int k = 0; k < 4; ++k) sum[t][k] *= EXACT ? Mma<T>::kExactUnit : Mma<T>::kUnit;
       if (wk == 1) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int c = 8 * t + 2 * quad + (k & 1), n = n0 + gid + 8 * (k >> 1);
-            if (c < cols && n < a.N && tile_of(at) < at.tile_end) store_result<T>(a, jobs.list[first + c], n, sum[t][k]);
+            if (c < cols && n < a.N && tile_of(at) < at.tile_end) store_result<T, EXACT>(a, jobs.list[first + c], n, sum[t][k]);
           }
       } else {
         // join the parts in order; the two halves of `red` alternate, so the one barrier of a round also ends the reads
@@ -476,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
           float v = 0.0f;
           for (int k = 0; k < wk; ++k) v += red[par][l * wk + k][c][r];
           const int n = (at.tile + at.round * at_once + l) * kTile + r;
-          if (n < a.N) store_result<T>(a, jobs.list[first + c], n, v);
+          if (n < a.N) store_result<T, EXACT>(a, jobs.list[first + c], n, v);
         }
         par ^= 1;
       }
@@ -484,17 +531,17 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
   }
 }
 
-template <typename T, int G, int NT, bool ZERO>
+template <typename T, int G, int NT, bool ZERO, bool EXACT>
 cudaError_t launch_kernel(MatvecArgs a, cudaStream_t stream) {
   constexpr size_t kRing = static_cast<size_t>(kWarps) * kDepth * Stage<G, ZERO>::kBytes;
   constexpr size_t kStatic = sizeof(float) * 2 * kWarps * 8 * NT * (kTile + 4) + sizeof(Jobs) + 4 * kWarps + 8 * 8 * NT;
   constexpr size_t kX = kSmemMost - kRing - kStatic - 1024 - kStep * 2;      // for staged x and its group sums
-  const auto kernel = matvec_w4_kernel<T, G, NT, ZERO>;
+  const auto kernel = matvec_w4_kernel<T, G, NT, ZERO, EXACT>;
   const int rows = a.pairs / a.per_row;             // a row that names an expert twice gives it a second job
   a.x_cols = rows < 8 * NT ? rows : 8 * NT;
   const int steps = (a.K + kStep - 1) / kStep;
   // steps that fit for one row, the sums of their groups, and the rest for staged rows, as much of it as the call can use
-  constexpr size_t kSums = static_cast<size_t>(kStep / G) * 8 * NT * 4;
+  constexpr size_t kSums = EXACT ? 0 : static_cast<size_t>(kStep / G) * 8 * NT * 4;
   const int most = static_cast<int>((kX - 64) / (kStep * 2 + kSums));
   a.slice_most = steps < most ? steps : most;
   size_t room = kX - a.slice_most * kSums;
@@ -509,16 +556,17 @@ cudaError_t launch_kernel(MatvecArgs a, cudaStream_t stream) {
   return launch_pdl(kernel, dim3(static_cast<unsigned>(items < kNumSMs ? items : kNumSMs)), dim3(kThreads), smem, stream, a);
 }
 
+template <typename T, int G, int NT>
+cudaError_t launch_kernel(const MatvecArgs& a, cudaStream_t stream) {
+  if (a.zero) return a.out_f32 ? launch_kernel<T, G, NT, true, true>(a, stream) : launch_kernel<T, G, NT, true, false>(a, stream);
+  return a.out_f32 ? launch_kernel<T, G, NT, false, true>(a, stream) : launch_kernel<T, G, NT, false, false>(a, stream);
+}
+
 template <typename T, int NT>
 cudaError_t launch_group(const MatvecArgs& a, int G, cudaStream_t stream) {
-  if (a.zero) {
-    if (G == 128) return launch_kernel<T, 128, NT, true>(a, stream);
-    if (G == 64) return launch_kernel<T, 64, NT, true>(a, stream);
-    return launch_kernel<T, 32, NT, true>(a, stream);
-  }
-  if (G == 128) return launch_kernel<T, 128, NT, false>(a, stream);
-  if (G == 64) return launch_kernel<T, 64, NT, false>(a, stream);
-  return launch_kernel<T, 32, NT, false>(a, stream);
+  if (G == 128) return launch_kernel<T, 128, NT>(a, stream);
+  if (G == 64) return launch_kernel<T, 64, NT>(a, stream);
+  return launch_kernel<T, 32, NT>(a, stream);
 }
 
 template <typename T>

@@ -503,12 +503,13 @@ def matvec_w4(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor, zero:
 
         out[r, n] = sum_k x[r, k] * (q[n, k] - zero[n, k // G]) * scale[n, k // G]
 
-    x bfloat16 / float16 [R, K] (bfloat16: |x| < 2^63); qweight uint8 [N, K / 2], two values a byte, the even k in the
+    x bfloat16 / float16 [R, K]; qweight uint8 [N, K / 2], two values a byte, the even k in the
     low half; scale [N, K / G] in x's type or float32, G = 32, 64 or 128; zero uint8 [N, K / G], 0 to 15 (None: 8).  With
     ``experts`` the weights have a leading dimension E and every (row, choice) has its own matrix: experts int32 [R] gives
     out [R, N], [R, k] gives [R, k, N] (the experts that ``route`` selected, less the shard's first); an expert outside
     [0, E) gives zeros.  At most 256 (row, choice) pairs and 1024 experts.  out has x's type, or float32 with
-    ``out_dtype``; sums are float32."""
+    ``out_dtype``; sums are float32.  For a float32 result q - zero is formed exactly; for a 16-bit one a group's sum is
+    sum q x - zero sum x, whose float32 errors go with sum |q x|, and bfloat16 wants |x| < 2^63."""
     dtype, dev, shape = x.dtype, x.device, x.shape
     if (dtype is not torch.bfloat16 and dtype is not torch.float16) or len(shape) != 2:
         raise ValueError("x must be bfloat16 or float16 [R, K]")

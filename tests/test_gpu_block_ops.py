@@ -509,6 +509,75 @@ def test_matvec_of_no_rows(op, g):
     assert op.matvec_w4(x, q, scale, experts=torch.empty((2, 0), dtype=torch.int32, device="cuda")).shape == (2, 0, 5)
 
 
+@pytest.mark.parametrize("t,ot", [(BF, F), (HF, F), (BF, None), (HF, None)])
+@pytest.mark.parametrize("R,N,K,G,zero,spread,E", [
+    (1, 512, 7168, 128, False, 1.5, 0), (5, 301, 2048, 64, True, 0.5, 0), (16, 128, 4096, 32, True, 0.3, 0),
+    (4, 96, 7168, 128, True, 0.2, 3), (16, 2001, 128, 128, False, 0.2, 0), (9, 999, 64, 64, True, 0.25, 2),
+])
+def test_matvec_of_weights_near_the_zero_point(op, g, R, N, K, G, zero, spread, E, t, ot):
+    """Trained weights lie close around the zero point, and activations have a mean and a few large channels: sum q x and
+    z sum x are then far larger than their difference, most of all where a large channel's weight is zero.  For an fp32 result q - z is exact and the error goes with sum |(q - z) x| all the same;
+    for a 16-bit one it goes with sum (q + z) |x|."""
+    x, q, scale, z = matvec_inputs(g, R, N, K, G, t, E, zero)
+    x = (x.float() + 1.0).to(t)
+    shape = ((E, N) if E else (N,)) + (K // G,)
+    zf = torch.full(shape, 8.0, device="cuda") if z is None else z.float()
+    v = (zf[..., None] + spread * torch.randn(shape + (G,), generator=g, device="cuda")).round().clamp(0, 15).to(torch.uint8)
+    v[..., 5] = zf
+    v = v.flatten(-2)
+    x[:, 5::G] *= 2.0 ** 12
+    q = (v[..., 0::2] | v[..., 1::2] << 4).contiguous()
+    e = torch.randint(0, E, (R, 2), generator=g, device="cuda", dtype=torch.int32) if E else None
+    out = op.matvec_w4(x, q, scale, z, experts=e, out_dtype=ot)
+
+    def ref(i, x):
+        at = (lambda v: v if v is None or i is None else v[i])  # noqa: E731
+        r, size = matvec_ref(x, at(q), at(scale), at(z))
+        if ot is None:
+            both = at(v).to(D) + at(zf).to(D).repeat_interleave(G, -1)
+            size = size + x.to(D).abs() @ (both * at(scale).to(D).abs().repeat_interleave(G, -1)).t()
+        return r, size
+    if not E:
+        near(out, *ref(None, x), MMA)
+        return
+    for r in range(R):
+        for k in range(2):
+            a, b = ref(int(e[r, k]), x[r:r + 1])
+            near(out[r, k], a[0], b[0], MMA)
+
+
+@pytest.mark.parametrize("t,sizes", [(BF, [2.0 ** 110, 2.0 ** 63, 1.0, 2.0 ** -57, 2.0 ** -100]), (HF, [2.0 ** 10, 1.0, 2.0 ** -10, 2.0 ** -20])])
+@pytest.mark.parametrize("zero", [False, True])
+def test_matvec_over_the_activations_range(op, g, t, sizes, zero):
+    """A row of every order of magnitude that the type has, each held to its own error."""
+    for f32 in (False, True):
+        x, q, scale, z = matvec_inputs(g, len(sizes), 130, 1024, 128, t, 0, zero, F if f32 else None)
+        x = (x.float() * torch.tensor(sizes, device="cuda")[:, None]).to(t)
+        near(op.matvec_w4(x, q, scale, z, out_dtype=F), *matvec_ref(x, q, scale, z), MMA)
+
+
+@pytest.mark.parametrize("zero", [False, True])
+def test_matvec_over_the_range_of_16_bit_results(op, g, zero):
+    """bf16 activations just below 2^63 and around 2^-57; fp16 ones as large as the result allows and subnormal."""
+    for t, sizes in ((BF, [2.0 ** 60, 2.0 ** 30, 2.0 ** -30, 2.0 ** -57]), (HF, [2.0 ** 8, 1.0, 2.0 ** -8, 2.0 ** -16])):
+        x, q, scale, z = matvec_inputs(g, 4, 130, 1024, 128, t, 0, zero)
+        x = (x.float() * torch.tensor(sizes, device="cuda")[:, None]).to(t)
+        if t is BF:
+            x[0, ::7] = 2.0 ** 63 * (1 - 2.0 ** -8)       # bf16's largest value below
+        near(op.matvec_w4(x, q, scale, z), *matvec_ref(x, q, scale, z), MMA)
+
+
+@pytest.mark.parametrize("t", [BF, HF])
+def test_matvec_of_infinite_activations(op, g, t):
+    """One infinite activation gives its weight's sign, and NaN where the weight is zero."""
+    x, q, scale, _ = matvec_inputs(g, 2, 40, 256, 64, t)
+    x[0, 9] = float("inf")
+    out = op.matvec_w4(x, q, scale.abs(), out_dtype=F)
+    w = (q[:, 4] >> 4).float() - 8
+    assert bool(out[0][w == 0].isnan().all()) and torch.equal(out[0][w != 0], w[w != 0] * float("inf"))
+    near(out[1], *(v[1] for v in matvec_ref(x, q, scale.abs(), None)), MMA)
+
+
 def test_matvec_infinities_stay_in_their_row(op, g):
     x, q, scale, _ = matvec_inputs(g, 3, 20, 256, 64, BF)
     x[1, 9] = float("inf")
