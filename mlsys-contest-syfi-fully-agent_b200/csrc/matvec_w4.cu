@@ -46,6 +46,7 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kDepth = 2;                  // stages of a warp's ring
 constexpr int kStep = 256;                 // columns of a stage
 constexpr int kTile = 16;                  // weight rows of an item
+constexpr int kSumSteps = 128;             // steps whose sums are added up in fp32 at most: off by 2^-17 of the terms
 constexpr int kSmemMost = 227 * 1024;
 
 struct MatvecArgs {
@@ -183,10 +184,10 @@ __device__ __forceinline__ void store_result(const MatvecArgs& a, int pair, int 
   else static_cast<T*>(a.out)[at] = from_f32<T>(v);
 }
 
-// sum += the products of a stage, 16 rows and 256 columns with USED of NT column tiles, times 1 / kUnit (kExactUnit).
+// total += the products of a stage, 16 rows and 256 columns with USED of NT column tiles, times 1 / kUnit (kExactUnit).
 template <typename T, int G, int USED, int NT, bool ZERO, bool EXACT>
 __device__ __forceinline__ void step(const MatvecArgs& a, const uint8_t* stage, const uint8_t* const (&x_at)[NT], const float* xs_at,
-                                     int u, const int (&s_at)[2], const int (&z_low)[2], int gid, int quad, float (&sum)[NT][4]) {
+                                     int u, const int (&s_at)[2], const int (&z_low)[2], int gid, int quad, float (&total)[NT][4]) {
   using S = Stage<G, ZERO>;
   constexpr int W = G / 32;                        // words of a lane per row and group
   // the scales of the lane's two rows; groups behind K have zeros for x and q and need a finite scale
@@ -207,6 +208,8 @@ __device__ __forceinline__ void step(const MatvecArgs& a, const uint8_t* stage, 
     for (int gi = 1; gi < S::kGroups; ++gi)
       if (u * kStep + gi * G >= a.K) scale[gi][0] = scale[gi][1] = 0.0f;
   }
+  float of_step[USED][4] = {};                     // many small groups: a sum of their own, which makes the long one shorter
+  auto sum = [&](int t, int i) -> float& { return G < 128 ? of_step[t][i] : total[t][i]; };
 #pragma unroll
   for (int gi = 0; gi < S::kGroups; ++gi) {
     typename Words<W>::Type w[2];
@@ -250,7 +253,7 @@ __device__ __forceinline__ void step(const MatvecArgs& a, const uint8_t* stage, 
 #pragma unroll
       for (int t = 0; t < USED; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[t][i] += (even[t][i] + odd[t][i]) * scale[gi][i >> 1];
+        for (int i = 0; i < 4; ++i) sum(t, i) += (even[t][i] + odd[t][i]) * scale[gi][i >> 1];
     } else {
       float2 xt[USED];
 #pragma unroll
@@ -262,11 +265,17 @@ __device__ __forceinline__ void step(const MatvecArgs& a, const uint8_t* stage, 
         if (ZERO) zero = static_cast<float>(stage[S::kZeros + r * 4 * S::kZeroWords + ((z_low[h] + u * S::kGroups) & 3) + gi]);
 #pragma unroll
         for (int t = 0; t < USED; ++t) {
-          sum[t][2 * h] += (even[t][2 * h] + 0.0625f * odd[t][2 * h] - zero * xt[t].x) * scale[gi][h];
-          sum[t][2 * h + 1] += (even[t][2 * h + 1] + 0.0625f * odd[t][2 * h + 1] - zero * xt[t].y) * scale[gi][h];
+          sum(t, 2 * h) += (even[t][2 * h] + 0.0625f * odd[t][2 * h] - zero * xt[t].x) * scale[gi][h];
+          sum(t, 2 * h + 1) += (even[t][2 * h + 1] + 0.0625f * odd[t][2 * h + 1] - zero * xt[t].y) * scale[gi][h];
         }
       }
     }
+  }
+  if (G < 128) {
+#pragma unroll
+    for (int t = 0; t < USED; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) total[t][i] += of_step[t][i];
   }
 }
 
@@ -495,6 +504,26 @@ __global__ void __launch_bounds__(kThreads, 1) matvec_w4_kernel(MatvecArgs a) {
           load(ring + slot * S::kBytes);
           slot = slot + 1 == kDepth ? 0 : slot + 1;
         }
+        if (steps > kSumSteps) {
+          // A long K comes in slices of up to kSumSteps: their sums meet in the thread's own places of `red`, with what the
+          // additions lose.  The barriers in front of every slice's x end the reads of the round before.
+          float *const all = &red[0][warp][0][0] + lane, *const lost = &red[1][warp][0][0] + lane;
+          static_assert(4 * NT * 32 <= kCols * (kTile + 4), "a warp's part of red holds its threads' sums");
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int i = (4 * t + k) * 32;
+              float v = at.slice > 0 ? all[i] : 0.0f, low = at.slice > 0 ? lost[i] : 0.0f;
+              add_exactly(v, low, sum[t][k]);
+              const bool done = at.slice == at.slices - 1;
+              sum[t][k] = done ? joined(v, low) : 0.0f;
+              if (done) continue;
+              all[i] = v;
+              lost[i] = low;
+            }
+          __syncwarp();
+        }
       }
 
 #pragma unroll
@@ -542,7 +571,7 @@ cudaError_t launch_kernel(MatvecArgs a, cudaStream_t stream) {
   const int steps = (a.K + kStep - 1) / kStep;
   // steps that fit for one row, the sums of their groups, and the rest for staged rows, as much of it as the call can use
   constexpr size_t kSums = EXACT ? 0 : static_cast<size_t>(kStep / G) * 8 * NT * 4;
-  const int most = static_cast<int>((kX - 64) / (kStep * 2 + kSums));
+  const int most = min(static_cast<int>((kX - 64) / (kStep * 2 + kSums)), kSumSteps);
   a.slice_most = steps < most ? steps : most;
   size_t room = kX - a.slice_most * kSums;
   const size_t useful = static_cast<size_t>(a.x_cols) * (a.slice_most * kStep * 2 + 64);

@@ -567,6 +567,24 @@ def test_matvec_over_the_range_of_16_bit_results(op, g, zero):
         near(op.matvec_w4(x, q, scale, z), *matvec_ref(x, q, scale, z), MMA)
 
 
+@pytest.mark.parametrize("R,N,K,G,t,E,k", [(1, 33, 2 ** 20, 32, BF, 0, 0), (16, 17, 2 ** 20, 128, HF, 0, 0), (9, 100, 2 ** 18 + 64, 64, BF, 0, 0),
+                                           (5, 20, 2 ** 17, 32, HF, 2, 3), (2, 40, 2 ** 15 + 32, 32, BF, 0, 0)])
+def test_matvec_of_long_rows(op, g, R, N, K, G, t, E, k):
+    """Equal activations and weights, so that all terms have one sign and every addition rounds the same way: a thread adds
+    at most 8 + 128 sums in a row, and 16 warps meet: 2^-17 of the sum with the few roundings of a group."""
+    x, q, scale, _ = matvec_inputs(g, R, N, K, G, t, E)
+    x = x[:, :1].abs().expand(R, K).contiguous()
+    scale = scale[..., :1].expand(scale.shape).contiguous().float()
+    q.fill_(13 * 17)
+    e = torch.randint(0, E, (R, k), generator=g, device="cuda", dtype=torch.int32) if E else None
+    out = op.matvec_w4(x, q, scale, experts=e, out_dtype=F)
+    for r in range(R):
+        for c in range(max(k, 1)):
+            w = scale[int(e[r, c])] if E else scale
+            ref = float(x[r, 0]) * 5 * K * w[:, 0].to(D)
+            near(out[r, c] if E else out[r], ref, ref.abs(), MMA)
+
+
 @pytest.mark.parametrize("t", [BF, HF])
 def test_matvec_of_infinite_activations(op, g, t):
     """One infinite activation gives its weight's sign, and NaN where the weight is zero."""
