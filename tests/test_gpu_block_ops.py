@@ -686,6 +686,31 @@ def test_on_a_stream_of_its_own(op, g):
     assert all(torch.equal(a, b) for a, b in zip(ref, got))
 
 
+def test_waits_for_what_its_stream_has_to_do_first(op, g):
+    """The inputs hold other values until a copy on the side stream, behind some milliseconds of work there, replaces them: a
+    call that ran on another stream or read too early would see the other values."""
+    call, inputs = every_call(op, g)
+    final = [t.clone() for t in inputs]
+    ref = [t.clone() for t in call()]
+    other = [torch.randn(t.shape, generator=g, device="cuda").to(t.dtype) for t in inputs]
+    for t, o in zip(inputs, other):
+        t.copy_(o)
+    stale = [t.clone() for t in call()]
+    assert sum(not torch.equal(a, b) for a, b in zip(ref, stale)) == len(ref) - 2      # all but counts and tokens
+    a = torch.randn((8192, 8192), generator=g, device="cuda").to(BF)
+    b = torch.empty_like(a)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(8):
+            torch.mm(a, a, out=b)
+        for t, f in zip(inputs, final):
+            t.copy_(f)
+        got = call()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(ref, got))
+
+
 def test_captured_and_replayed(op, g):
     """Two graphs of the same calls, replayed in turn on new inputs, give what ordinary calls give."""
     call, inputs = every_call(op, g)
