@@ -19,7 +19,7 @@ namespace {
 // copies exactly the sixteen-byte pieces that it will read itself, so the ring needs no barrier.  Weights come from the
 // first-level cache, which the copies pass by.  A thread has sixteen columns of a row of 4096 and more: two CTAs of 448
 // threads at 7168 columns, whose barriers fill each other's gaps.
-// Measured, 4096 x 7168 bf16: join and norm 47 us (5.0 TB/s), with e4m3 output 50 us (4.2 TB/s: 61 % of the issue slots
+// Measured, 4096 x 7168 bf16: join and norm 47 us (5.0 TB/s), with e4m3 output 51 us (4.1 TB/s: 61 % of the issue slots
 // are taken, the conversion's maximum and products among them); without the ring 79 us.  4096 x 5001 (kEdges) 44 us, with
 // rows 5006 apart (kShifted) 59 us, element by element 180 us.
 //
@@ -175,20 +175,31 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 3 : CH
       for (int j = 0; j < 4; ++j) s[c][j] = mul2(mul2(s[c][j], rr), w[j]);
       if (QUANT) {
         // sixteen lanes hold a block of 128 columns; scale = max(|h|, 1e-10) / 448 and e4m3(h / scale), the rule of the
-        // activation quantiser, with products of reciprocals (errors of 2^-22 before the rounding to e4m3's 2^-4)
+        // activation quantiser and the same bits.  Both quotients are products with a reciprocal, corrected by what they leave
+        // of the dividend.  For the constant that is the rounded quotient of every fp32 value (checked for all mantissas; the
+        // method is Brisebarre, Muller and Raina's of 2004); for the values it is but for ties of fp32, and no quotient of
+        // fp32 values lies that close to a tie of e4m3 without being one
         const int col = column<true>(c, 0);
         float amax = 1e-10f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fmaxf(fabsf(get(s[c][j]).x), fabsf(get(s[c][j]).y)));
 #pragma unroll
         for (int d = 8; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
-        const float scale = amax * (1.0f / 448.0f);
-        const F2 inverse = both(__fdividef(1.0f, scale));
+        const float about = amax * (1.0f / 448.0f);
+        const bool finite = about < INFINITY;              // an infinite block: zeros, NaN where it is infinite
+        const float scale = finite ? fmaf(fmaf(-448.0f, about, amax), 1.0f / 448.0f, about) : about;
+        const F2 inverse = both(__fdividef(1.0f, scale)), minus = both(finite ? -scale : 0.0f);
         uint32_t packed[2];
+        float2 quotient[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const F2 near = mul2(s[c][j], inverse);
+          quotient[j] = get(fma2(fma2(minus, near, s[c][j]), inverse, near));
+        }
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-          packed[j] = __nv_cvt_float2_to_fp8x2(get(mul2(s[c][2 * j], inverse)), __NV_SATFINITE, __NV_E4M3) |
-                      static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(get(mul2(s[c][2 * j + 1], inverse)), __NV_SATFINITE, __NV_E4M3)) << 16;
+          packed[j] = __nv_cvt_float2_to_fp8x2(quotient[2 * j], __NV_SATFINITE, __NV_E4M3) |
+                      static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(quotient[2 * j + 1], __NV_SATFINITE, __NV_E4M3)) << 16;
         if (col < H) {
           *reinterpret_cast<uint2*>(q_out + col) = make_uint2(packed[0], packed[1]);
           if ((threadIdx.x & 15) == 0) a.q_scale[static_cast<int64_t>(col / kBlock) * a.T + row] = scale;

@@ -255,6 +255,32 @@ def test_block_norm_quantized(op, g, T, H, t, gate):
     assert float(q.to(F).abs().max()) == 448.0
 
 
+def test_block_norm_quantizes_as_the_activation_quantiser_does(op, g):
+    """Rows of +-1 keep their norm factor at 1, so h is the weights with signs, exactly, and both ways to the shard's input
+    see the same values: the same scales and codes."""
+    for k in range(20):
+        x = torch.where(torch.rand((33, 7168), generator=g, device="cuda") < 0.5, -1.0, 1.0).to(BF)
+        w = torch.randn(7168, generator=g, device="cuda") * 2.0 ** torch.randint(-12, 12, (7168,), generator=g, device="cuda")
+        w[::128] = 448.0 * 2.0 ** (k - 10)                 # quotients of few bits, ties of e4m3 among them
+        w = w.to(BF)
+        _, (q, scale), rstd = op.block_norm(x, w, eps=1e-30, quantize=True)
+        assert bool((rstd[:, 1] == 1).all())
+        want_q, want_scale = op.quantize_activations((x.float() * w.float()).to(BF))
+        assert torch.equal(scale, want_scale)
+        assert torch.equal(q.view(torch.uint8), want_q.view(torch.uint8))
+
+
+def test_block_norm_quantized_infinite_values(op):
+    """One infinite value of h: its block has an infinite scale, zeros, and NaN in its place."""
+    x = torch.ones((2, 256), device="cuda")
+    w = torch.ones(256, device="cuda")
+    w[3] = float("inf")
+    q, scale = op.block_norm(x, w, quantize=True)[1]
+    v = q.to(F)
+    assert bool(scale[0].isinf().all()) and bool(v[:, 3].isnan().all()) and bool((v[:, 128:] == 448).all())
+    assert not bool(v[:, :3].any()) and not bool(v[:, 4:128].any())
+
+
 def test_block_norm_quantized_zero_rows(op):
     q, scale = op.block_norm(torch.zeros((2, 256), device="cuda"), torch.ones(256, device="cuda"), quantize=True)[1]
     assert not bool(q.to(F).any())
