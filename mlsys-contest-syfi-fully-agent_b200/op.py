@@ -362,8 +362,8 @@ def block_norm(x: torch.Tensor, pre_weight: torch.Tensor, y: Optional[torch.Tens
     [H / 128, T]) that ``run`` takes as hidden_states and hidden_states_scale, rounded from the unrounded h; H must then
     be a multiple of 128 and all rows 16-byte aligned.  Arithmetic is float32, what is stored is rounded once."""
     T, H, args = _norm_inputs(x, pre_weight, y, post_weight, gate, residual_scale)
-    if not eps > 0.0:
-        raise ValueError("eps must be positive")
+    if not eps >= 2.0 ** -149:
+        raise ValueError("eps must be a positive float32")
     if quantize:
         if H % BLOCK != 0:
             raise ValueError(f"quantize needs a multiple of {BLOCK} columns")

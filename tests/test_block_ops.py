@@ -221,3 +221,9 @@ def test_launches_on_the_tensors_device_with_its_stream(op, monkeypatch, getters
     assert seen == [(1, (7, 8, 101))] and state["device"] == current
     with pytest.raises(op.loader.MoeLibraryError):
         op._launch(lambda *args: op.loader.EINVAL, torch.device("cuda", 1))
+
+
+@pytest.mark.parametrize("eps", [1e-60, 0.0, -1e-6, float("nan")])
+def test_block_norm_refuses_an_eps_that_fp32_does_not_hold(op, eps):
+    with pytest.raises(ValueError, match="eps"):
+        op.block_norm(**norm_args(), eps=eps)
