@@ -103,7 +103,7 @@ __device__ __forceinline__ void probabilities(const BalanceArgs& a, const Raw<T,
     for (int i = 0; i < EPL; ++i) {
       const float z = expert_of<T, VEC>(i, lane) < a.E ? to_f32<T>(r.v[i]) : -INFINITY;
       const float x = expf(-z);
-      p[i] = __fdividef(1.0f, 1.0f + x);
+      p[i] = __fdividef(1.0f, 1.0f + x);                 // 2 units in the last place at most
       if (x > 0x1p125f) p[i] = 0.0f;                     // beyond the fast division's range; the row is shifted if it matters
       if (SLOPE) slope[i] = z > 0.0f ? x * p[i] : 1.0f - p[i];
       sum += p[i];
@@ -436,6 +436,7 @@ cudaError_t launch_chunks(const BalanceArgs& a, bool backward, cudaStream_t stre
   }
   if (per_lane <= 2) return launch_chunks<T, 2, false>(a, backward, stream);
   if (per_lane <= 8) return launch_chunks<T, 8, false>(a, backward, stream);
+  // 257 to 512 experts too: a kernel between the two was not measured
   return launch_chunks<T, 32, false>(a, backward, stream);
 }
 

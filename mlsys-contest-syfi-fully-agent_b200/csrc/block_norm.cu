@@ -175,10 +175,10 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : kNormThreads, CH == 1 ? 3 : CH
       for (int j = 0; j < 4; ++j) s[c][j] = mul2(mul2(s[c][j], rr), w[j]);
       if (QUANT) {
         // sixteen lanes hold a block of 128 columns; scale = max(|h|, 1e-10) / 448 and e4m3(h / scale), the rule of the
-        // activation quantiser and the same bits.  Both quotients are products with a reciprocal, corrected by what they leave
-        // of the dividend.  For the constant that is the rounded quotient of every fp32 value (checked for all mantissas; the
-        // method is Brisebarre, Muller and Raina's of 2004); for the values it is but for ties of fp32, and no quotient of
-        // fp32 values lies that close to a tie of e4m3 without being one
+        // activation quantiser and the same values (a zero loses its sign).  Both quotients are products with a reciprocal,
+        // corrected by what they leave of the dividend.  For the constant that is the rounded quotient of every fp32 value
+        // (checked for all mantissas; the method is Brisebarre, Muller and Raina's of 2004); for the values it is but for
+        // ties of fp32, and no quotient of fp32 values lies that close to a tie of e4m3 without being one
         const int col = column<true>(c, 0);
         float amax = 1e-10f;
 #pragma unroll

@@ -28,10 +28,10 @@
 // stages of 16 rows x 256 columns a warp, 64 KB in flight per SM), which run on across items.  A warp has an item to
 // itself, or several warps share its K when there are too few items; then their sums meet in shared memory in a fixed
 // order.  (A ring in registers waits for its newest loads with its oldest: 97 us where this takes 31.)
-// Measured, bf16, groups of 128: one token through eight 4096 x 7168 experts 31 us (3.8 TB/s of weights), sixteen tokens'
-// second products through 7168 x 2048 experts 57 us (3.8 TB/s), sixteen tokens through all 32 first ones 115 us (4.2 TB/s);
+// Measured, bf16, groups of 128: one token through eight 4096 x 7168 experts 32 us (3.7 TB/s of weights), sixteen tokens'
+// second products through 7168 x 2048 experts 57 us (3.8 TB/s), sixteen tokens through all 32 first ones 110 us (4.4 TB/s);
 // half of the issue slots are taken, and what is left is the latency of unpacking and products with four warps on each
-// quarter of an SM.  Deeper rings change nothing, 24 warps of 80 registers take 39 us instead of 31.
+// quarter of an SM.  Deeper rings change nothing, 24 warps of 80 registers take 39 us instead of 32.
 #include <limits.h>
 
 #include "elem_device.cuh"

@@ -509,7 +509,7 @@ def matvec_w4(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor, zero:
     out [R, N], [R, k] gives [R, k, N] (the experts that ``route`` selected, less the shard's first); an expert outside
     [0, E) gives zeros.  At most 256 (row, choice) pairs and 1024 experts.  out has x's type, or float32 with
     ``out_dtype``; sums are float32.  For a float32 result q - zero is formed exactly; for a 16-bit one a group's sum is
-    sum q x - zero sum x, whose float32 errors go with sum |q x|, and bfloat16 wants |x| < 2^63."""
+    sum q x - zero sum x, whose float32 errors go with sum |q x|, and bfloat16 wants |x| < 2^63 (an infinite x gives NaN)."""
     dtype, dev, shape = x.dtype, x.device, x.shape
     if (dtype is not torch.bfloat16 and dtype is not torch.float16) or len(shape) != 2:
         raise ValueError("x must be bfloat16 or float16 [R, K]")
